@@ -83,17 +83,17 @@ def draw(rng):
                     rng.random() < 0.7, rng.random() < 0.3)
     elif op == "cache":
         heads, dim = rng.choice([1, 2, 4, 8, 12]), rng.choice([64, 96, 128, 256])
-        read = max(2, min(_spread(rng, 16, 65536), 65536 * 8 * 128 // (heads * dim * 2)))
-        c = _cache("", min(read, _spread(rng, 1, 8192)), read, heads, dim, rng.choice([1, 8, 16, 32, 64, 128]), rng.choice(["bf16", "fp16", "fp32"]),
+        read = max(2, min(_spread(rng, 16, 65536), 60000 * 8 * 128 // (heads * dim * 2)))
+        c = _cache("", min(read, _spread(rng, 1, 8192)), read, heads, dim, rng.choice([8, 16, 32, 64, 128]), rng.choice(["bf16", "fp16", "fp32"]),
                    rng.choice(["int8", "e4m3", "e4m3", "int8", "bf16", "fp16"]))
     elif op == "paged":
         dtype = rng.choice(["bf16", "fp16"])
         dim, hk = rng.choice([64, 96, 128, 256]), rng.choice([1, 2, 4, 8, 12])
         hq = hk * rng.choice([1, 2, 4, 5, 8, 16])
         long = _spread(rng, 1, 131072)
-        batch = max(1, min(_spread(rng, 1, 256), 270000 * 8 * 128 // (long * hk * dim)))
-        if batch * long * max(hk * dim, hq * 32) > 270000 * 8 * 128:
-            long = max(1, 270000 * 8 * 128 // (batch * max(hk * dim, hq * 32)))
+        batch = max(1, min(_spread(rng, 1, 256), 260000 * 8 * 128 // (long * hk * dim)))
+        if batch * long * max(hk * dim, hq * 32) > 260000 * 8 * 128:
+            long = max(1, 260000 * 8 * 128 // (batch * max(hk * dim, hq * 32)))
         c = _paged("", batch, _spread(rng, 1, long), long, hq, hk, dim, rng.choice([8, 16, 32, 64, 128]), dtype,
                    rng.choice([dtype, dtype, "int8", "e4m3"]), rng.choice([0.0, 0.0, 30.0, 50.0]), rng.choice([0, 0, _spread(rng, 64, 4096)]),
                    rng.random() < 0.25)
