@@ -14,11 +14,15 @@ there is no CPU fallback.
   FlatIndex           resident HBM index + fused inner-product/top-k search
   SparseIndex, Splade resident CSR index + exact sparse search; SPLADE plug-in (models.retrievers.splade.Splade)
   merge_topk          device merge of per-shard partial top-k lists
+  qk_norm_rotary, kv_cache, kv_cache_write, kv_cache_read, paged_attention, token_logprobs, rotary_frequencies
+                      operators of a decoding step (device tensors, current stream)
   ShardedSearcher     row-sharded multi-GPU search (one process per GPU, RCCL all-gather)
   utils               chunk-file / .trec formats, path naming (reference utils.py)
 """
 from . import evaluation, utils  # noqa: F401
 from .config import instantiate  # noqa: F401
+from .decoding import (KVCache, TokenLogprobs, kv_cache, kv_cache_read, kv_cache_write, paged_attention, qk_norm_rotary,  # noqa: F401
+                       rotary_frequencies, token_logprobs)
 from .dense import ClsPooler, CosineSim, Dense, DotProduct, MeanPooler, Retriever  # noqa: F401
 from .encoder import BertEncoder  # noqa: F401
 from .index import FlatIndex, merge_topk  # noqa: F401

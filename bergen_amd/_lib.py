@@ -13,7 +13,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("BERGEN_HIP_LIB", os.path.join(_HERE, "lib", "libbergen_hip.so"))
 
-BH_VERSION = 143  # the header version the struct layouts below mirror (tests/test_abi.py compares it with include/bergen_hip.h)
+BH_VERSION = 144  # the header version the struct layouts below mirror (tests/test_abi.py compares it with include/bergen_hip.h)
 
 BH_OK = 0
 BH_EINVAL = -1
@@ -24,6 +24,9 @@ BH_EUNSUPPORTED = -5
 
 BH_F16 = 0
 BH_F32 = 1
+BH_BF16 = 2
+BH_I8 = 3
+BH_E4M3 = 4
 BH_METRIC_IP = 0
 BH_METRIC_COS = 1
 
@@ -142,6 +145,15 @@ SYMBOLS = {
     "bh_op_rotary": (ctypes.c_int, [_vp, _i64, _i32, _vp, ctypes.c_float, _i32]),
     "bh_op_swiglu": (ctypes.c_int, [_vp, _vp, _i64, _i32]),
     "bh_op_gated_act": (ctypes.c_int, [_vp, _vp, _i64, _i32, _i32]),
+    "bh_op_qk_norm_rotary": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _i64, _i32, _i32, _i32,
+                                            _i32, _vp, _i32, _vp, _vp, _vp, _i32, ctypes.c_float, _i32, _vp]),
+    "bh_op_kv_write": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _vp]),
+    "bh_op_kv_read": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _vp]),
+    "bh_op_paged_attention_workspace": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "bh_op_paged_attention": (ctypes.c_int, [_vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _vp, _i64, _i32, _vp, _i32, _i32, _i32,
+                                             _i32, ctypes.c_float, ctypes.c_float, _i32, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "bh_op_token_logprobs_workspace": (_i64, [_i64, _i64, _i32, _i32]),
+    "bh_op_token_logprobs": (ctypes.c_int, [_vp, _i64, _i32, _i64, _i64, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "bh_gemm_permlane_mode": (ctypes.c_int, []),
     "bh_sparse_create": (ctypes.c_int, [ctypes.POINTER(_vp), _i64, _i32]),
     "bh_sparse_upload_csr": (ctypes.c_int, [_vp, _i64, _i64, _vp, _vp, _vp, _i32]),

@@ -1,0 +1,555 @@
+// paged_attention.hip — attention of one new token per sequence over a paged key-value cache, split over the cache's length.
+//
+//   s_t = scale q . k_t;  capped: s = c tanh(s / c);  distance bias: s -= slope (len - 1 - t);  t in [max(0, len - window), len)
+//   out = sum_t e^(s_t - m) v_t / sum_t e^(s_t - m),   lse = m + log sum_t e^(s_t - m)       (nothing left: out 0, lse -inf)
+//
+// Bound: HBM, by the cache's bytes — each key and value is read once for the whole group of query heads that shares it.  A query
+// head alone makes 1 flop per byte, a group of 8 makes 8; on the vector units 8 would already take all their cycles, so both products run
+// on the matrix cores, 16 heads wide whether there are 16 or 1 (24 MFMAs of 16 cycles for 16 KiB of cache are 4 % of the time
+// that HBM needs for them).
+//
+// A wave takes 32 tokens of one key head at a time and needs no LDS for them:
+//   S^T = K Q^T     two tiles of 16 tokens.  Row i of tile u is token 8 (i / 4) + 4 u + i % 4, so that lane (g, n) — g = lane / 16,
+//                   n = lane % 16 — ends up with the scores of the 8 CONSECUTIVE tokens 8 g .. 8 g + 7 of head n;
+//   O^T += V^T P^T  wants in lane (g, n) the weights of 8 tokens of head n: those 8, as they are.  Its V^T operand, lane (g, i),
+//                   wants the same 8 tokens of one dim; the lane loads D / 16 consecutive dims of each of them (a group's 16 lanes: a
+//                   whole row) and turns its own little block round with byte permutes.
+// Keys: lane (g, i) loads 16 bytes of its row, groups side by side.  8-bit codes become fp16, exactly, between load and
+// MFMA; the keys' scale multiplies the score, the values' scale the weight.
+// Weights reach the MFMA as a sum of two numbers of its type (hi + lo): bf16 alone would keep 2^-9 of a weight, as much as
+// the output's own rounding.  fp16 weights are held times 2^14 so that small ones do not become subnormal.
+//
+// Pages are 8..1024 tokens (a power of two): 8 consecutive tokens share one.  A table entry outside [0, pages) names a page that is
+// not there: its tokens are left out.  What lies behind a sequence's end is neither counted nor multiplied (its values
+// are replaced by zeros: 0 x NaN is NaN).
+#include <type_traits>
+
+#include "bh_decode.h"
+
+namespace {
+
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr int WAVES = 4, TILE = 32;
+
+struct PagedArgs {
+    const void* q;
+    long long q_seq, q_head;  // strides in elements
+    void* out;                // [batch][hq][dim]
+    float* lse;               // [batch][hq] or null
+    const void *k, *v;
+    const float *k_scale, *v_scale, *slopes;
+    const int* table;
+    long long table_stride;
+    const int* lengths;
+    float* part_stats;  // [batch][hq][splits][2]: m log2(e), sum
+    float* part_out;    // [batch][hq][splits][dim], not yet divided
+    int batch, hq, hk, group, blocks, dim, n_pages, page_log2, table_width;
+    int splits, per_split;  // per_split: tokens, a multiple of WAVES * TILE
+    int window;
+    float scale, softcap;
+};
+
+template <typename E>
+struct Mma;
+template <>
+struct Mma<_Float16> {
+    typedef half8 frag;
+    static __device__ __forceinline__ floatx4 mul(frag a, frag b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Mma<__bf16> {
+    typedef bf16x8 frag;
+    static __device__ __forceinline__ floatx4 mul(frag a, frag b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+
+__device__ __forceinline__ float over_groups_max(float v) {  // over the 4 lanes with the same lane % 16
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float over_groups_sum(float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+// two codes (bits 0..7 and 16..23 of `pair`, or any two bytes chosen by `sel`) -> two fp16
+template <int CACHE>
+__device__ __forceinline__ unsigned two_f16(unsigned word, int which) {
+    if (CACHE == BH_I8) {
+        // 1024 + (code + 128) as fp16 is the byte 0x64 over the code with its top bit flipped; minus 1152 is exact
+        const unsigned u = word ^ 0x80808080u;
+        const unsigned w = __builtin_amdgcn_perm(0x64646464u, u, which ? 0x04030402u : 0x04010400u);
+        half2v h = __builtin_bit_cast(half2v, w);
+        h -= (half2v){(_Float16)1152.f, (_Float16)1152.f};
+        return __builtin_bit_cast(unsigned, h);
+    }
+    return which ? __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.0f, true))
+                 : __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.0f, false));
+}
+
+// E: the queries' type; CACHE: BH_F16 / BH_BF16 (E's own), BH_I8, BH_E4M3; DP: head dim, rounded up to 64, 128 or 256.
+template <typename E, int CACHE, int DP>
+__global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) bh_paged_attention_kernel(PagedArgs a) {
+    constexpr bool SCALED = CACHE == BH_I8 || CACHE == BH_E4M3;
+    typedef typename std::conditional<SCALED, _Float16, E>::type M;  // the MFMAs' type
+    typedef typename Mma<M>::frag frag;
+    constexpr int ES = SCALED ? 1 : 2;            // bytes of a cached element
+    constexpr int KS = DP / 32;                   // steps of S^T
+    constexpr int KL = KS * 8 * ES / 16;          // 16-byte loads of a key row per lane
+    constexpr int NJ = DP / 16;                   // dims of a value row per lane = tiles of O^T
+    constexpr int VW = NJ * ES / 4;               // their words
+    constexpr bool F16 = std::is_same<M, _Float16>::value;
+    constexpr float HOLD = F16 ? 14.f : 0.f;      // weights are held times 2^HOLD
+
+    __shared__ float sh_stats[WAVES][2][16];
+    __shared__ float sh_out[WAVES][16][DP + 4];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, n = lane & 15;
+    const int split = blockIdx.x, seq = blockIdx.z;
+    const int hk = blockIdx.y / a.blocks, block = blockIdx.y - hk * a.blocks;
+    const int hq0 = hk * a.group + 16 * block;                       // the first of this workgroup's query heads
+    const int heads = a.group - 16 * block < 16 ? a.group - 16 * block : 16;
+
+    int len = a.lengths[seq];
+    const long long most = (long long)a.table_width << a.page_log2;
+    len = len < 0 ? 0 : len > most ? (int)most : len;
+    const int start = a.window > 0 && len > a.window ? len - a.window : 0;
+    const int first = start & ~(TILE - 1);
+    const int live_splits = (len - first + a.per_split - 1) / a.per_split;
+    if (split >= live_splits && split > 0) return;
+    const int lo = first + split * a.per_split;
+    const int hi = lo + a.per_split < len ? lo + a.per_split : len;
+
+    // ---- the queries, operand B of S^T: lane (g, n) holds head n, dims as its key chunks
+    const bool head_live = n < heads;
+    const E* qp = static_cast<const E*>(a.q) + seq * a.q_seq + (long long)(hq0 + (head_live ? n : 0)) * a.q_head;
+    frag qf[KS];
+    float unit = a.scale * LOG2E;  // of a score, in powers of two
+    {
+        float top = 0.f;
+        bf16x8 qb[KS];
+        (void)qb;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = SCALED ? 16 * ((s >> 1) * 4 + g) + 8 * (s & 1) : 8 * (4 * s + g);
+            typedef E vec __attribute__((ext_vector_type(8)));
+            vec x = {};
+            if (head_live && d < a.dim) x = *reinterpret_cast<const vec*>(qp + d);
+            if constexpr (std::is_same<E, M>::value) {
+                qf[s] = __builtin_bit_cast(frag, x);
+            } else {
+                qb[s] = x;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf((float)x[e]));
+            }
+        }
+        if constexpr (!std::is_same<E, M>::value) {
+            // bf16 queries against 8-bit keys: as fp16, times the power of two that brings the head's largest to 2^7..2^8 (exact above
+            // 2^-22 of it)
+            top = over_groups_max(top);
+            int e = (int)(__float_as_uint(top) >> 23) - 127;
+            e = e > 126 ? 126 : e < -112 ? -112 : e;
+            const float up = ldexpf(1.f, 7 - e);
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) qf[s][i] = (_Float16)((float)qb[s][i] * up);
+            unit *= ldexpf(1.f, e - 7);
+        }
+    }
+    const float slope = a.slopes && head_live ? a.slopes[hq0 + n] * LOG2E : 0.f;
+    const float cap = a.softcap * LOG2E, cap_unit = a.softcap > 0.f ? 2.f / a.softcap : 0.f;
+
+    float m, total;  // of head n: the same m in its 4 lanes, each lane's own sum
+    float v_top;     // values' scales are held against a power of two
+    floatx4 o[NJ];
+
+    const int* table = a.table + seq * a.table_stride;
+    const unsigned char* kc = static_cast<const unsigned char*>(a.k);
+    const unsigned char* vc = static_cast<const unsigned char*>(a.v);
+    const long long row = (long long)a.dim * ES;
+    const int in_page = (1 << a.page_log2) - 1;
+
+    // the vector of token t in the cache (its index), if its page is there; t is a multiple of 8
+    auto vector_at = [&](int t, bool& there) {
+        const int page = t < len ? table[t >> a.page_log2] : -1;
+        there = page >= 0 && page < a.n_pages;
+        return ((((long long)(there ? page : 0) * a.hk + hk) << a.page_log2) + (there ? t & in_page : 0));
+    };
+
+    // lo can be zero or below: an infinite value, times it, spoils what hi made of it.  Where a sum came out as NaN, the walk is taken once
+    // more with hi alone, for those sums only
+    bool both = true;
+    for (;; both = false) {
+        m = -INFINITY, total = 0.f, v_top = 0x1p-126f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) o[j] = floatx4{0.f, 0.f, 0.f, 0.f};
+        for (int t0 = lo + wave * TILE; t0 < hi; t0 += WAVES * TILE) {
+            bool there, key_there;
+            const long long kv = vector_at(t0 + 8 * (n >> 2), key_there) + (n & 3);  // keys of row n: + 4 in the second tile
+            const long long vv = vector_at(t0 + 8 * g, there);                       // the lane's 8 tokens
+            uint4 kr[2][KL];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int s = 0; s < KL; ++s) {
+                    const int byte = 16 * (4 * s + g);
+                    kr[u][s] = uint4{0, 0, 0, 0};
+                    if (key_there && byte < row) kr[u][s] = *reinterpret_cast<const uint4*>(kc + (kv + 4 * u) * row + byte);
+                }
+            unsigned vreg[8][VW];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+#pragma unroll
+                for (int w = 0; w < VW; ++w) vreg[r][w] = 0;
+                const bool want = there && t0 + 8 * g + r < hi && t0 + 8 * g + r >= start && NJ * n < a.dim;
+                if (want) {
+                    const unsigned char* p = vc + (vv + r) * row + NJ * ES * n;
+                    if constexpr (VW == 1) {
+                        vreg[r][0] = *reinterpret_cast<const unsigned*>(p);
+                    } else if constexpr (VW == 2) {
+                        const uint2 x = *reinterpret_cast<const uint2*>(p);
+                        vreg[r][0] = x.x, vreg[r][1] = x.y;
+                    } else {
+#pragma unroll
+                        for (int w = 0; w < VW; w += 4) {
+                            const uint4 x = *reinterpret_cast<const uint4*>(p + 4 * w);
+                            vreg[r][w] = x.x, vreg[r][w + 1] = x.y, vreg[r][w + 2] = x.z, vreg[r][w + 3] = x.w;
+                        }
+                    }
+                }
+            }
+            float ks[8], vs[8];
+            if constexpr (SCALED) {
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    ks[r] = there ? a.k_scale[vv + r] : 0.f;
+                    vs[r] = there && t0 + 8 * g + r < hi && t0 + 8 * g + r >= start ? a.v_scale[vv + r] : 0.f;
+                }
+            }
+
+            // ---- S^T
+            floatx4 st[2] = {floatx4{0.f, 0.f, 0.f, 0.f}, floatx4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    frag kf;
+                    if constexpr (SCALED) {
+                        const uint4 c = kr[u][s >> 1];
+                        const unsigned w0 = s & 1 ? c.z : c.x, w1 = s & 1 ? c.w : c.y;
+                        const uint4 f = {two_f16<CACHE>(w0, 0), two_f16<CACHE>(w0, 1), two_f16<CACHE>(w1, 0), two_f16<CACHE>(w1, 1)};
+                        kf = __builtin_bit_cast(frag, f);
+                    } else {
+                        kf = __builtin_bit_cast(frag, kr[u][s]);
+                    }
+                    st[u] = Mma<M>::mul(kf, qf[s], st[u]);
+                }
+
+            // ---- softmax: the lane's 8 tokens of head n
+            float x[8];
+            float top = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                const int t = t0 + 8 * g + r;
+                float dot = st[r >> 2][r & 3];
+                if constexpr (SCALED) dot *= ks[r];
+                float y = dot * unit;
+                if (a.softcap > 0.f) {
+                    const float e2 = __builtin_amdgcn_exp2f(fminf(y * cap_unit, 64.f));  // e^(2 s / c)
+                    y = y == y ? cap * (e2 - 1.f) * __builtin_amdgcn_rcpf(e2 + 1.f) : y;
+                }
+                y -= slope * (float)(len - 1 - t);
+                x[r] = there && t < hi && t >= start ? y : -INFINITY;
+                top = fmaxf(top, x[r]);
+            }
+            const float now = fmaxf(m, over_groups_max(top));
+            const float base = now == -INFINITY ? 0.f : now;
+            float fade = __builtin_amdgcn_exp2f(m - base);
+            m = now;
+            float per = 1.f;
+            if constexpr (SCALED) {
+                float big = vs[0];
+#pragma unroll
+                for (int r = 1; r < 8; ++r) big = fmaxf(big, vs[r]);
+                big = over_groups_max(big);
+                // the power of two at or above it
+                const unsigned b = __float_as_uint(big);
+                const float up = __uint_as_float((b & 0x7f800000u) + ((b & 0x7fffffu) && b < 0x7f000000u ? 0x800000u : 0u));
+                const float next = fmaxf(v_top, up);
+                const float shrink = v_top / next;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) o[j] *= shrink;
+                v_top = next;
+                per = 1.f / next;
+            }
+            float p[8];
+            total *= fade;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                p[r] = __builtin_amdgcn_exp2f(x[r] - base);
+                total += p[r];
+                p[r] *= (F16 ? 0x1p14f : 1.f);
+                if constexpr (SCALED) p[r] *= vs[r] * per;
+            }
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) o[j] *= fade;
+            frag hi_p, lo_p;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                // one value for both: left alone, the compiler rounds the product above to fp16 once in a fused instruction for hi and once
+                // by way of fp32 for what hi is subtracted from, and where those fall on different sides lo belongs to another hi
+                asm("" : "+v"(p[r]));
+                hi_p[r] = (M)p[r];
+                lo_p[r] = both ? (M)(p[r] - (float)hi_p[r]) : (M)0.f;
+            }
+
+            // ---- O^T
+            if constexpr (SCALED) {
+#pragma unroll
+                for (int w = 0; w < VW; ++w) {  // 4 dims of 8 tokens
+                    unsigned f[4][4];
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {  // tokens 2 h, 2 h + 1
+                        const unsigned e01 = __builtin_amdgcn_perm(vreg[2 * h + 1][w], vreg[2 * h][w], 0x05010400u);
+                        const unsigned e23 = __builtin_amdgcn_perm(vreg[2 * h + 1][w], vreg[2 * h][w], 0x07030602u);
+                        f[0][h] = two_f16<CACHE>(e01, 0);
+                        f[1][h] = two_f16<CACHE>(e01, 1);
+                        f[2][h] = two_f16<CACHE>(e23, 0);
+                        f[3][h] = two_f16<CACHE>(e23, 1);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const frag vf = __builtin_bit_cast(frag, (uint4{f[e][0], f[e][1], f[e][2], f[e][3]}));
+                        o[4 * w + e] = Mma<M>::mul(vf, hi_p, o[4 * w + e]);
+                        o[4 * w + e] = Mma<M>::mul(vf, lo_p, o[4 * w + e]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int w = 0; w < VW; ++w) {  // 2 dims of 8 tokens
+                    uint4 f0, f1;
+                    f0.x = __builtin_amdgcn_perm(vreg[1][w], vreg[0][w], 0x05040100u), f1.x = __builtin_amdgcn_perm(vreg[1][w], vreg[0][w], 0x07060302u);
+                    f0.y = __builtin_amdgcn_perm(vreg[3][w], vreg[2][w], 0x05040100u), f1.y = __builtin_amdgcn_perm(vreg[3][w], vreg[2][w], 0x07060302u);
+                    f0.z = __builtin_amdgcn_perm(vreg[5][w], vreg[4][w], 0x05040100u), f1.z = __builtin_amdgcn_perm(vreg[5][w], vreg[4][w], 0x07060302u);
+                    f0.w = __builtin_amdgcn_perm(vreg[7][w], vreg[6][w], 0x05040100u), f1.w = __builtin_amdgcn_perm(vreg[7][w], vreg[6][w], 0x07060302u);
+                    const frag v0 = __builtin_bit_cast(frag, f0), v1 = __builtin_bit_cast(frag, f1);
+                    o[2 * w] = Mma<M>::mul(v0, hi_p, o[2 * w]);
+                    if (both) o[2 * w] = Mma<M>::mul(v0, lo_p, o[2 * w]);
+                    o[2 * w + 1] = Mma<M>::mul(v1, hi_p, o[2 * w + 1]);
+                    if (both) o[2 * w + 1] = Mma<M>::mul(v1, lo_p, o[2 * w + 1]);
+                }
+            }
+        }
+        if (SCALED || !both) break;
+        bool odd = false;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) odd |= o[j][r] != o[j][r];
+        if (!__any(odd)) break;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sh_out[wave][n][NJ * (4 * g + r) + j] = o[j][r];
+    }
+
+    // ---- the workgroup's waves joined
+    total = over_groups_sum(total);
+    if (g == 0) {
+        sh_stats[wave][0][n] = m;
+        sh_stats[wave][1][n] = total;
+    }
+    __syncthreads();
+    float all = sh_stats[0][0][n];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) all = fmaxf(all, sh_stats[w][0][n]);
+    const float base = all == -INFINITY ? 0.f : all;
+    const float mine = __builtin_amdgcn_exp2f(m - base - HOLD) * (SCALED ? v_top : 1.f);
+    // lane (g, n), tile j, element r: head n, dim NJ (4 g + r) + j
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            float& to = sh_out[wave][n][NJ * (4 * g + r) + j];
+            const float x = !SCALED && !both && to == to ? to : o[j][r];
+            to = m == -INFINITY ? 0.f : x * mine;
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < heads * a.dim; i += 64 * WAVES) {
+        const int h = i / a.dim, d = i - h * a.dim;
+        float top = sh_stats[0][0][h], sum = 0.f, x = 0.f;
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) top = fmaxf(top, sh_stats[w][0][h]);
+        const float from = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            sum += sh_stats[w][1][h] * __builtin_amdgcn_exp2f(sh_stats[w][0][h] - from);
+            x += sh_out[w][h][d];
+        }
+        const long long at = (long long)seq * a.hq + hq0 + h;
+        if (live_splits > 1) {
+            a.part_out[(at * a.splits + split) * a.dim + d] = x;
+            if (d == 0) {
+                a.part_stats[2 * (at * a.splits + split)] = top;
+                a.part_stats[2 * (at * a.splits + split) + 1] = sum;
+            }
+        } else {
+            static_cast<E*>(a.out)[at * a.dim + d] = (E)(sum > 0.f || sum != sum ? x / sum : 0.f);
+            if (d == 0 && a.lse) a.lse[at] = sum > 0.f || sum != sum ? LN2 * (top + __builtin_amdgcn_logf(sum)) : -INFINITY;
+        }
+    }
+}
+
+// Joins the splits of one query head: a workgroup a head, thread d its dim (and the splits by turns, where there are threads left).
+template <typename E>
+__global__ void __launch_bounds__(256) bh_paged_attention_join_kernel(PagedArgs a) {
+    __shared__ float sh[256];
+    __shared__ float sh_sum;
+    const int head = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x;
+    int len = a.lengths[seq];
+    const long long most = (long long)a.table_width << a.page_log2;
+    len = len < 0 ? 0 : len > most ? (int)most : len;
+    const int start = a.window > 0 && len > a.window ? len - a.window : 0;
+    const int live = (len - (start & ~(TILE - 1)) + a.per_split - 1) / a.per_split;
+    if (live <= 1) return;  // written by its only workgroup
+    const long long at = (long long)seq * a.hq + head;
+    const float* stats = a.part_stats + 2 * at * a.splits;
+    float top = -INFINITY;
+    for (int s = tid; s < live; s += 256) top = fmaxf(top, stats[2 * s]);
+    for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+    if ((tid & 63) == 0) sh[tid >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
+    const float from = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    for (int s = tid; s < live; s += 256) sum += stats[2 * s + 1] * __builtin_amdgcn_exp2f(stats[2 * s] - from);
+    sum = bh_group_sum(sum, 64);
+    __syncthreads();
+    if ((tid & 63) == 0) sh[tid >> 6] = sum;
+    __syncthreads();
+    if (tid == 0) sh_sum = sh[0] + sh[1] + sh[2] + sh[3];
+    __syncthreads();
+    sum = sh_sum;
+    const int wide = 1 << (32 - __clz(a.dim - 1));  // threads of one split: a power of two, 16..256
+    const int d = tid & (wide - 1), turns = 256 / wide;
+    float x = 0.f;
+    if (d < a.dim)
+        for (int s = tid / wide; s < live; s += turns)
+            x += a.part_out[(at * a.splits + s) * a.dim + d] * __builtin_amdgcn_exp2f(stats[2 * s] - from);
+    sh[tid] = x;
+    __syncthreads();
+    if (tid < a.dim) {
+        for (int i = 1; i < turns; ++i) x += sh[tid + i * wide];
+        static_cast<E*>(a.out)[at * a.dim + tid] = (E)(sum > 0.f || sum != sum ? x / sum : 0.f);
+        if (tid == 0 && a.lse) a.lse[at] = sum > 0.f || sum != sum ? LN2 * (top + __builtin_amdgcn_logf(sum)) : -INFINITY;
+    }
+}
+
+// How the cache's length is split: about 2048 workgroups (8 on each CU) at the longest that the table allows, in splits of 128 tokens
+// and more; a sequence uses as many of them as its own length fills.
+void split_length(int64_t batch, int64_t blocks, int64_t longest, int32_t window, int* splits, int* per_split) {
+    if (window > 0 && window + TILE < longest) longest = window + TILE;  // (a window's start is rounded down to a tile)
+    const int64_t step = WAVES * TILE, work = batch * blocks;
+    int64_t want = (2048 + work - 1) / work;
+    int64_t per = (longest + want - 1) / want;
+    per = (per + step - 1) / step * step;
+    if (per < step) per = step;
+    if (per < 512 && longest > 512 && work * ((longest + 511) / 512) >= 512) per = 512;
+    *per_split = (int)per;
+    const int64_t n = (longest + per - 1) / per;
+    *splits = (int)(n < 1 ? 1 : n);
+}
+
+template <typename E, int CACHE>
+void launch_dim(const PagedArgs& a, hipStream_t st) {
+    const dim3 grid(a.splits, a.hk * a.blocks, a.batch), block(64 * WAVES);
+    if (a.dim <= 64)
+        hipLaunchKernelGGL((bh_paged_attention_kernel<E, CACHE, 64>), grid, block, 0, st, a);
+    else if (a.dim <= 128)
+        hipLaunchKernelGGL((bh_paged_attention_kernel<E, CACHE, 128>), grid, block, 0, st, a);
+    else
+        hipLaunchKernelGGL((bh_paged_attention_kernel<E, CACHE, 256>), grid, block, 0, st, a);
+    if (a.splits > 1) hipLaunchKernelGGL((bh_paged_attention_join_kernel<E>), dim3(a.hq, a.batch), dim3(256), 0, st, a);
+}
+
+int check_sizes(int32_t batch, int32_t hq, int32_t hk, int32_t dim, int32_t page_size, int32_t width) {
+    if (batch < 0 || hq <= 0 || hk <= 0 || width < 0) return bh_fail(BH_EINVAL, "bad sizes");
+    if (hq % hk) return bh_fail(BH_EINVAL, "%d query heads on %d key heads", hq, hk);
+    if (dim < 16 || dim > 256 || dim % 16) return bh_fail(BH_EUNSUPPORTED, "head_dim %d (a multiple of 16, 16..256)", dim);
+    if (page_size < 8 || page_size > 1024 || (page_size & (page_size - 1)))
+        return bh_fail(BH_EUNSUPPORTED, "page_size %d (a power of two, 8..1024)", page_size);
+    if (batch > 65535 || hq > 65535 || (long long)width * page_size > (1 << 30))
+        return bh_fail(BH_EUNSUPPORTED, "more than 65535 sequences or heads, or 2^30 tokens of a sequence");
+    return BH_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t bh_op_paged_attention_workspace(int32_t batch, int32_t n_q_heads, int32_t n_k_heads, int32_t head_dim, int32_t page_size,
+                                        int32_t table_width, int32_t window) {
+    const int rc = check_sizes(batch, n_q_heads, n_k_heads, head_dim, page_size, table_width);
+    if (rc) return rc;
+    if (window < 0) return bh_fail(BH_EINVAL, "bad window");
+    if (batch == 0) return 0;
+    int splits, per;
+    split_length(batch, (int64_t)n_k_heads * ((n_q_heads / n_k_heads + 15) / 16), (int64_t)table_width * page_size, window, &splits, &per);
+    return splits > 1 ? (int64_t)batch * n_q_heads * splits * (2 + (int64_t)head_dim) * 4 : 0;
+}
+
+int bh_op_paged_attention(const void* q, int64_t q_seq, int64_t q_head, int32_t dtype, const void* k_cache, const void* v_cache,
+                          const float* k_scale, const float* v_scale, int32_t cache_dtype, int64_t n_pages, int32_t page_size,
+                          const int32_t* table, int64_t table_stride, int32_t table_width, const int32_t* lengths, int32_t batch,
+                          int32_t n_q_heads, int32_t n_k_heads, int32_t head_dim, float scale, float softcap, int32_t window,
+                          const float* slopes, void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+    const int rc = check_sizes(batch, n_q_heads, n_k_heads, head_dim, page_size, table_width);
+    if (rc) return rc;
+    if (dtype != BH_F16 && dtype != BH_BF16) return bh_fail(BH_EINVAL, "bad dtype %d (fp16 or bf16)", dtype);
+    const bool scaled = cache_dtype == BH_I8 || cache_dtype == BH_E4M3;
+    if (!scaled && cache_dtype != dtype) return bh_fail(BH_EINVAL, "bad cache dtype %d (the queries' own %d, int8 or e4m3)", cache_dtype, dtype);
+    if (!(scale == scale) || !(softcap >= 0.f) || softcap == __builtin_inff() || window < 0)
+        return bh_fail(BH_EINVAL, "bad scale, softcap or window");
+    if (n_pages < 0 || n_pages > 0x7fffffff) return bh_fail(BH_EINVAL, "bad sizes");
+    if (batch == 0) return BH_OK;
+    if (!q || !lengths || !out || (table_width && (!table || !k_cache || !v_cache))) return bh_fail(BH_EINVAL, "null buffer");
+    if (scaled && table_width && (!k_scale || !v_scale)) return bh_fail(BH_EINVAL, "an 8-bit cache needs the scales of keys and values");
+    if (!bh_aligned16(q) || !bh_aligned16(k_cache) || !bh_aligned16(v_cache) || (q_seq | q_head) % 8)
+        return bh_fail(BH_EUNSUPPORTED, "queries and cache must be 16-byte aligned");
+    PagedArgs a{};
+    a.group = n_q_heads / n_k_heads;
+    a.blocks = (a.group + 15) / 16;
+    split_length(batch, (int64_t)n_k_heads * a.blocks, (int64_t)table_width * page_size, window, &a.splits, &a.per_split);
+    const int64_t parts = a.splits > 1 ? (int64_t)batch * n_q_heads * a.splits : 0, need = parts * (2 + (int64_t)head_dim) * 4;
+    if (need && (!workspace || workspace_bytes < need || !bh_aligned16(workspace)))
+        return bh_fail(BH_EINVAL, "workspace of %lld bytes, 16-byte aligned, needed: %lld given", (long long)need, (long long)workspace_bytes);
+    a.q = q, a.q_seq = q_seq, a.q_head = q_head, a.out = out, a.lse = lse;
+    a.k = k_cache, a.v = v_cache, a.k_scale = k_scale, a.v_scale = v_scale, a.slopes = slopes;
+    a.table = table, a.table_stride = table_stride, a.lengths = lengths;
+    a.part_out = static_cast<float*>(workspace);
+    a.part_stats = a.part_out + parts * head_dim;
+    a.batch = batch, a.hq = n_q_heads, a.hk = n_k_heads, a.dim = head_dim, a.n_pages = (int)n_pages;
+    a.page_log2 = bh_ceil_log2(page_size), a.table_width = table_width;
+    a.window = window, a.scale = scale, a.softcap = softcap;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (dtype == BH_F16) {
+        if (cache_dtype == BH_F16)
+            launch_dim<_Float16, BH_F16>(a, st);
+        else if (cache_dtype == BH_I8)
+            launch_dim<_Float16, BH_I8>(a, st);
+        else
+            launch_dim<_Float16, BH_E4M3>(a, st);
+    } else {
+        if (cache_dtype == BH_BF16)
+            launch_dim<__bf16, BH_BF16>(a, st);
+        else if (cache_dtype == BH_I8)
+            launch_dim<__bf16, BH_I8>(a, st);
+        else
+            launch_dim<__bf16, BH_E4M3>(a, st);
+    }
+    BH_HIP_TRY(hipGetLastError());
+    return BH_OK;
+}
+
+}  // extern "C"

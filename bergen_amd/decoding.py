@@ -1,0 +1,257 @@
+"""
+Operators of a decoding step on hand-written HIP kernels: what a decoder that answers from the retrieved passages, or scores them by
+the log probability of a token, runs next to its matrix products (the reference reaches such models through
+AutoModelForCausalLM, models/generators/llm.py).
+
+  rotary_frequencies   the rotary positions' inverse frequencies, in 64 bits (made once)
+  qk_norm_rotary       RMS norm of each query / key head and rotary positions, in one pass
+  kv_cache             an empty paged key-value cache: fp16, bf16, int8 or e4m3
+  kv_cache_write       keys and values into their slots, quantised on the way
+  kv_cache_read        slots back as vectors
+  paged_attention      attention of one new token per sequence over that cache
+  token_logprobs       log probabilities of given tokens, entropy, likeliest alternatives
+
+They take device tensors, ENQUEUE on the current stream of the tensors' device and return (the other entry points of this package wait); they can
+be captured into a graph.  They run inference only: a tensor that requires a gradient is refused while gradients are recorded.
+"""
+import collections
+import ctypes
+
+import torch
+
+from . import _lib
+
+_FLOATS = {torch.float16: _lib.BH_F16, torch.bfloat16: _lib.BH_BF16, torch.float32: _lib.BH_F32}
+_CACHES = {torch.float16: _lib.BH_F16, torch.bfloat16: _lib.BH_BF16, torch.int8: _lib.BH_I8, torch.float8_e4m3fn: _lib.BH_E4M3}
+_SCALED = (torch.int8, torch.float8_e4m3fn)
+
+TokenLogprobs = collections.namedtuple("TokenLogprobs", "logprobs entropy top_logprobs top_ids")
+
+_ready = set()
+
+
+def _need(ok, message):
+    if not ok:
+        raise ValueError(message)
+
+
+def _same_device(first, **others):
+    """Every tensor on one GPU, and none that waits for a gradient; -> that device."""
+    device = first.device
+    _need(device.type == "cuda", f"tensors must be on the GPU, got one on {device}")
+    grad = torch.is_grad_enabled()
+    _need(not (grad and first.requires_grad), "no backward pass here: call under torch.no_grad()")
+    for name, t in others.items():
+        if t is not None:
+            _need(t.device == device, f"{name} is on {t.device}, expected {device}")
+            _need(not (grad and t.requires_grad), f"{name} requires a gradient and there is no backward pass here: call under torch.no_grad()")
+    if device.index not in _ready:
+        with torch.cuda.device(device):
+            _lib.init(device.index)  # once per device: is it a gfx950 part
+        _ready.add(device.index)
+    return device
+
+
+def _call(device, fn, *args):
+    """fn(*args, stream) with the tensors' device as the current one, on its current stream."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device.index:
+        _lib.check(fn(*args, stream))
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn(*args, stream))
+
+
+def _rows(name, t, heads=None, dim=None):
+    """[tokens, heads, dim] with the last dimension dense."""
+    _need(t.dim() == 3, f"{name} must be [tokens, heads, dim], got {tuple(t.shape)}")
+    _need(t.dtype in _FLOATS, f"{name} must be float16, bfloat16 or float32, got {t.dtype}")
+    _need((heads is None or t.shape[1] == heads) and (dim is None or t.shape[2] == dim), f"{name} has shape {tuple(t.shape)}")
+    _need(t.shape[2] <= 1 or t.stride(2) == 1, f"{name}'s last dimension must be dense")
+
+
+def _distinct(name, t):
+    """An output whose elements share no memory (an expanded view would)."""
+    room = 1
+    for size, stride in sorted(zip(t.shape, t.stride()), key=lambda p: p[1]):
+        if size > 1:
+            _need(stride >= room, f"{name} overlaps itself (shape {tuple(t.shape)}, strides {t.stride()}): it cannot be written")
+            room = stride * size
+
+
+def rotary_frequencies(rotary_dim, theta=10000.0, scale=1.0, device="cuda"):
+    """inv_freq[j] = scale * theta^(-2 j / rotary_dim), j < rotary_dim / 2, float64: what `qk_norm_rotary` turns a pair by, per position."""
+    _need(rotary_dim >= 0 and rotary_dim % 2 == 0, f"rotary_dim must be even, got {rotary_dim}")
+    j = torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device)
+    return float(scale) * float(theta) ** (-j / max(1, rotary_dim))
+
+
+def qk_norm_rotary(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, inplace=False):
+    """RMS norm of each head of q [tokens, n_q, dim] and k [tokens, n_k, dim], then rotary positions, in one pass -> (q, k).
+
+    positions [tokens] int32 / int64; inv_freq [rotary_dim / 2] float64 (`rotary_frequencies`): the pair (j, j + rotary_dim / 2) — or (2 j, 2 j + 1)
+    with interleaved — is turned by positions * inv_freq[j]; elements behind rotary_dim stay.  q_weight, k_weight [dim], of q's type
+    or float32; None: that side is not normalised.  q and k are float16, bfloat16 or float32, any strides with a dense last
+    dimension (slices of one projection).  inplace: into q and k themselves.
+    """
+    _rows("q", q)
+    _rows("k", k, dim=q.shape[2])
+    tokens, nq, dim = q.shape
+    _need(k.dtype == q.dtype and k.shape[0] == tokens, f"k must be [{tokens}, heads, {dim}] {q.dtype}, got {tuple(k.shape)} {k.dtype}")
+    _need(positions.shape == (tokens,) and positions.dtype in (torch.int32, torch.int64), f"positions must be int32 or int64 [{tokens}]")
+    _need(inv_freq.dim() == 1 and inv_freq.dtype == torch.float64 and 2 * inv_freq.numel() <= dim,
+          f"inv_freq must be float64 [rotary_dim / 2], rotary_dim at most {dim}")
+    wtype = None
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None:
+            _need(w.shape == (dim,) and w.dtype in (q.dtype, torch.float32), f"{name} must be [{dim}], {q.dtype} or float32")
+            _need(wtype in (None, w.dtype), "q_weight and k_weight must have one type")
+            _need(w.is_contiguous(), f"{name} must be contiguous")
+            wtype = w.dtype
+    _need(positions.is_contiguous() and inv_freq.is_contiguous(), "positions and inv_freq must be contiguous")
+    if inplace:
+        _distinct("q", q)
+        _distinct("k", k)
+    device = _same_device(q, k=k, positions=positions, inv_freq=inv_freq, q_weight=q_weight, k_weight=k_weight)
+    qo, ko = (q, k) if inplace else (torch.empty(q.shape, dtype=q.dtype, device=device), torch.empty(k.shape, dtype=k.dtype, device=device))
+    _call(device, _lib.lib().bh_op_qk_norm_rotary, q.data_ptr(), q.stride(0), q.stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1),
+          k.data_ptr(), k.stride(0), k.stride(1), ko.data_ptr(), ko.stride(0), ko.stride(1), _FLOATS[q.dtype], tokens, nq, k.shape[1], dim,
+          2 * inv_freq.numel(), positions.data_ptr(), int(positions.dtype == torch.int64), inv_freq.data_ptr(),
+          q_weight.data_ptr() if q_weight is not None else None, k_weight.data_ptr() if k_weight is not None else None,
+          _FLOATS[wtype or q.dtype], float(eps), int(bool(interleaved)))
+    return qo, ko
+
+
+KVCache = collections.namedtuple("KVCache", "k_cache v_cache k_scale v_scale")
+
+
+def kv_cache(pages, heads, page_size, dim, dtype=torch.bfloat16, device="cuda"):
+    """An empty paged cache -> KVCache(k_cache, v_cache [pages, heads, page_size, dim], k_scale, v_scale [pages, heads, page_size] or None)."""
+    _need(dtype in _CACHES, f"a cache holds float16, bfloat16, int8 or float8_e4m3fn, got {dtype}")
+    shape = (pages, heads, page_size, dim)
+    made = [torch.zeros(shape, dtype=torch.int8 if dtype in _SCALED else dtype, device=device).view(dtype) for _ in range(2)]
+    scales = [torch.zeros(shape[:3], dtype=torch.float32, device=device) if dtype in _SCALED else None for _ in range(2)]
+    return KVCache(*made, *scales)
+
+
+def _cache_tensors(k_cache, v_cache, k_scale, v_scale):
+    _need(k_cache.dim() == 4 and k_cache.dtype in _CACHES, f"k_cache must be [pages, heads, page_size, dim], float16, bfloat16, int8 or float8_e4m3fn; "
+          f"got {tuple(k_cache.shape)} {k_cache.dtype}")
+    _need(v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype, "v_cache must have k_cache's shape and type")
+    _need(k_cache.is_contiguous() and v_cache.is_contiguous(), "k_cache and v_cache must be contiguous")
+    if k_cache.dtype in _SCALED:
+        for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
+            _need(s is not None and s.shape == k_cache.shape[:3] and s.dtype == torch.float32 and s.is_contiguous(),
+                  f"an 8-bit cache needs {name}: contiguous float32 {tuple(k_cache.shape[:3])}")
+    else:
+        _need(k_scale is None and v_scale is None, f"a cache of {k_cache.dtype} has no scales")
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def kv_cache_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
+    """Rows k, v [tokens, heads, dim] (float16, bfloat16 or float32) into their slots (int64 [tokens]; page * page_size + offset) of the cache.
+
+    A slot outside the cache, -1 for padding, is skipped; the slots of one call must differ.  8-bit caches: int8 with scale = amax / 127 and the
+    exact quotient rounded to nearest even; float8_e4m3fn with the least power of two that keeps amax within 448.  A vector that holds an
+    infinity or a NaN reads back as NaN.
+    """
+    _cache_tensors(k_cache, v_cache, k_scale, v_scale)
+    pages, heads, page, dim = k_cache.shape
+    _rows("k", k, heads, dim)
+    _rows("v", v, heads, dim)
+    _need(v.shape == k.shape and v.dtype == k.dtype, "v must have k's shape and type")
+    _need(slots.shape == (k.shape[0],) and slots.dtype == torch.int64 and slots.is_contiguous(), f"slots must be contiguous int64 [{k.shape[0]}]")
+    device = _same_device(k, v=v, slots=slots, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale)
+    _call(device, _lib.lib().bh_op_kv_write, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _FLOATS[k.dtype],
+          slots.data_ptr(), k.shape[0], heads, dim, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), _CACHES[k_cache.dtype],
+          pages, page)
+
+
+def kv_cache_read(slots, k_cache, v_cache, k_scale=None, v_scale=None, dtype=torch.bfloat16):
+    """The slots' keys and values (int64 [tokens]) as `dtype` -> (k, v) [tokens, heads, dim]; zeros for a slot outside the cache."""
+    _cache_tensors(k_cache, v_cache, k_scale, v_scale)
+    pages, heads, page, dim = k_cache.shape
+    _need(dtype in _FLOATS, f"dtype must be float16, bfloat16 or float32, got {dtype}")
+    _need(slots.dim() == 1 and slots.dtype == torch.int64 and slots.is_contiguous(), "slots must be contiguous int64 [tokens]")
+    device = _same_device(slots, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale)
+    k, v = (torch.empty((slots.shape[0], heads, dim), dtype=dtype, device=device) for _ in range(2))
+    _call(device, _lib.lib().bh_op_kv_read, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _FLOATS[dtype],
+          slots.data_ptr(), slots.shape[0], heads, dim, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale),
+          _CACHES[k_cache.dtype], pages, page)
+    return k, v
+
+
+def paged_attention(q, k_cache, v_cache, block_table, lengths, scale=None, k_scale=None, v_scale=None, softcap=0.0, window=0,
+                    alibi_slopes=None, return_lse=False):
+    """Attention of one new token per sequence over a paged cache: q [batch, n_q, dim] -> out, or (out, lse) with return_lse.
+
+    q is float16 or bfloat16, dim a multiple of 16 up to 256; the cache (`kv_cache`) q's type, int8 or float8_e4m3fn with its scales;
+    n_q a multiple of the cache's heads.  lengths [batch] int32: tokens of each sequence in the cache, its newest among them;
+    block_table [batch, width] int32: their pages in order.  A length is taken as 0 .. width * page_size, and the tokens of an entry
+    outside the cache's pages are left out.  scale: 1 / sqrt(dim) unless given.  softcap c > 0: scores c tanh(s / c).  alibi_slopes [n_q]
+    float32: minus slope times the distance.  window w > 0: the last w tokens only.  lse [batch, n_q] float32: log of the sum of e^score.
+    A sequence with nothing left gives zeros and -inf.
+    """
+    _cache_tensors(k_cache, v_cache, k_scale, v_scale)
+    pages, heads, page, dim = k_cache.shape
+    _rows("q", q, dim=dim)
+    batch, nq, _ = q.shape
+    _need(q.dtype in (torch.float16, torch.bfloat16), f"q must be float16 or bfloat16, got {q.dtype}")
+    _need(k_cache.dtype == q.dtype or k_cache.dtype in _SCALED, f"the cache must be {q.dtype}, int8 or float8_e4m3fn, got {k_cache.dtype}")
+    _need(block_table.dim() == 2 and block_table.shape[0] == batch and block_table.dtype == torch.int32
+          and (block_table.shape[1] <= 1 or block_table.stride(1) == 1), f"block_table must be int32 [{batch}, width] with dense rows")
+    _need(lengths.shape == (batch,) and lengths.dtype == torch.int32 and lengths.is_contiguous(), f"lengths must be contiguous int32 [{batch}]")
+    if alibi_slopes is not None:
+        _need(alibi_slopes.shape == (nq,) and alibi_slopes.dtype == torch.float32 and alibi_slopes.is_contiguous(),
+              f"alibi_slopes must be contiguous float32 [{nq}]")
+    device = _same_device(q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, lengths=lengths, k_scale=k_scale, v_scale=v_scale,
+                          alibi_slopes=alibi_slopes)
+    if q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8:
+        q = q.contiguous()
+    lib, width = _lib.lib(), block_table.shape[1]
+    need = lib.bh_op_paged_attention_workspace(batch, nq, heads, dim, page, width, int(window))
+    if need < 0:
+        _lib.check(need)
+    out = torch.empty((batch, nq, dim), dtype=q.dtype, device=device)
+    lse = torch.empty((batch, nq), dtype=torch.float32, device=device) if return_lse else None
+    # (made anew for each call: two calls at once, or two captured graphs, must not share one)
+    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _call(device, lib.bh_op_paged_attention, q.data_ptr(), q.stride(0), q.stride(1), _FLOATS[q.dtype], k_cache.data_ptr(), v_cache.data_ptr(),
+          _ptr(k_scale), _ptr(v_scale), _CACHES[k_cache.dtype], pages, page, block_table.data_ptr(), block_table.stride(0), width,
+          lengths.data_ptr(), batch, nq, heads, dim, float(dim ** -0.5 if scale is None else scale), float(softcap), int(window),
+          _ptr(alibi_slopes), out.data_ptr(), _ptr(lse), _ptr(work), need)
+    return (out, lse) if return_lse else out
+
+
+def token_logprobs(logits, targets, top=0):
+    """Log probabilities of given tokens, entropy and the `top` likeliest tokens of each row, in one pass over logits [rows, vocab].
+
+    logits: float16, bfloat16 or float32 with dense rows; targets: int64 [rows] or [rows, given].  -> TokenLogprobs(logprobs float32 of targets'
+    shape, entropy float32 [rows] in nats, top_logprobs float32 and top_ids int64 [rows, top] in the order logit descending, id ascending).
+    A negative target's log probability is 0 (padding), one beyond the vocabulary NaN.  -inf logits carry no probability; a row of nothing
+    else has log probabilities -inf and entropy 0; a row with a NaN or +inf has NaN.  top is at most 64.
+    """
+    _need(logits.dim() == 2 and logits.dtype in _FLOATS, f"logits must be [rows, vocab], float16, bfloat16 or float32; got {tuple(logits.shape)} {logits.dtype}")
+    rows, vocab = logits.shape
+    _need(vocab >= 1 and (vocab == 1 or logits.stride(1) == 1), "logits' rows must be dense and not empty")
+    _need(targets.dtype == torch.int64 and targets.dim() in (1, 2) and targets.shape[0] == rows and targets.is_contiguous(),
+          f"targets must be contiguous int64 [{rows}] or [{rows}, given]")
+    device = _same_device(logits, targets=targets)
+    if rows > 1 and logits.stride(0) < vocab:
+        logits = logits.contiguous()
+    lib, top = _lib.lib(), int(top)
+    need = lib.bh_op_token_logprobs_workspace(rows, vocab, _FLOATS[logits.dtype], top)
+    if need < 0:
+        _lib.check(need)
+    logprobs = torch.empty(targets.shape, dtype=torch.float32, device=device)
+    entropy = torch.empty((rows,), dtype=torch.float32, device=device)
+    top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=device)
+    top_ids = torch.empty((rows, top), dtype=torch.int64, device=device)
+    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _call(device, lib.bh_op_token_logprobs, logits.data_ptr(), logits.stride(0), _FLOATS[logits.dtype], rows, vocab, targets.data_ptr(),
+          1 if targets.dim() == 1 else targets.shape[1], top, logprobs.data_ptr(), entropy.data_ptr(), top_logprobs.data_ptr(),
+          top_ids.data_ptr(), _ptr(work), need)
+    return TokenLogprobs(logprobs, entropy, top_logprobs, top_ids)

@@ -11,7 +11,8 @@
  *   - every function returns 0 on success or a negative bh_status; it never throws;
  *     a thread-local message is available from bh_last_error().
  *   - host buffers are owned by the caller and must stay alive for the duration of the
- *     call; all calls are synchronous (they return after the device work has finished).
+ *     call; all calls are synchronous (they return after the device work has finished), except the
+ *     operators that take a `stream`.
  *   - device memory and the opaque bh_index are owned by the library.
  *   - matrices are row-major, C-contiguous.
  *   - there is NO CPU fallback in this library: without a HIP device bh_init fails.
@@ -39,8 +40,10 @@ extern "C" {
  * (whether the last forward pass ran with the LayerNorms fused into the GEMM epilogues: encoder option "ln_fused") and bh_counters grew
  * balanced_scan_ms / balanced_queries at its END (option balance_tail); 143 = 0.1.4.3 (round 6): bh_encoder_config grew rotary_scale at its
  * END and accepts activation 0 with ffn_gated 1 (the GELU-gated feed-forward + NTK-scaled rotary positions of Alibaba-NLP/gte-*-en-v1.5,
- * config/retriever/gte-base-en-v1.5.yaml), alibi (jina-embeddings-v2) + bh_op_gated_act (bh_op_swiglu with the gate's activation as an argument). */
-#define BH_VERSION 143
+ * config/retriever/gte-base-en-v1.5.yaml), alibi (jina-embeddings-v2) + bh_op_gated_act (bh_op_swiglu with the gate's activation as an argument).
+ * 144 = 0.1.4.4: + the operators of a decoding step (bh_op_qk_norm_rotary, bh_op_kv_write, bh_op_kv_read, bh_op_paged_attention,
+ * bh_op_token_logprobs and two workspace queries) and three more values of bh_dtype; no struct changed. */
+#define BH_VERSION 144
 
 typedef enum bh_status {
     BH_OK = 0,
@@ -51,7 +54,8 @@ typedef enum bh_status {
     BH_EUNSUPPORTED = -5 /* unsupported k / dim / dtype */
 } bh_status;
 
-typedef enum bh_dtype { BH_F16 = 0, BH_F32 = 1 } bh_dtype;
+/* (BH_BF16, BH_I8 and BH_E4M3 — since BH_VERSION 144 — are types of the decoding operators only: every other entry point keeps refusing them) */
+typedef enum bh_dtype { BH_F16 = 0, BH_F32 = 1, BH_BF16 = 2, BH_I8 = 3, BH_E4M3 = 4 } bh_dtype;
 typedef enum bh_metric {
     BH_METRIC_IP = 0, /* DotProduct.sim, reference models/retrievers/dense.py:77-81 */
     BH_METRIC_COS = 1 /* CosineSim.sim,  reference models/retrievers/dense.py:83-89 */
@@ -343,6 +347,61 @@ int bh_op_layernorm(const void* in, void* out, int64_t n_rows, int32_t d, float 
                     const void* beta);
 /* 0 / 1 = direction of v_permlane32_swap found on the device (diagnostic), -1 on failure. */
 int bh_gemm_permlane_mode(void);
+
+/* Operators of a decoding step ---------------------------------------------------------------
+ * What a decoder that answers from the retrieved passages, or scores them by the log probability of a token, runs next to its
+ * matrix products (the reference reaches those models through AutoModelForCausalLM, models/generators/llm.py).  All pointers are DEVICE pointers.  Unlike the calls above these ENQUEUE on
+ * `stream` (a hipStream_t; NULL = the null stream) and return; they allocate nothing, keep nothing from one call for the next, and can be captured
+ * into a graph.  A workspace belongs to one call at a time.  Strides are in elements; a stride of the last dimension is 1.  Nothing here has a backward pass. */
+
+/* RMS norm of each query / key head and rotary positions, in one pass.  q [n_tokens][n_q_heads][head_dim], k likewise, of dtype
+ * (fp16, bf16, fp32): y = x / sqrt(mean(x^2) + eps) * weight (a NULL weight: y = x), then the pair (y[j], y[j + rotary_dim / 2]), j <
+ * rotary_dim / 2 — or (y[2 j], y[2 j + 1]) with interleaved != 0 — is turned by positions[token] * inv_freq[j] radians (fp64: the
+ * angle is formed in 64 bits); elements behind rotary_dim (even, may be 0) stay.  One rounding at the end.  Weights: dtype's own or fp32, [head_dim].  positions: int32, or int64 with
+ * positions_i64 != 0.  head_dim 1..256.  The outputs may be the inputs themselves (same pointer and strides) and must not overlap them otherwise. */
+int bh_op_qk_norm_rotary(const void* q, int64_t q_tok, int64_t q_head, void* q_out, int64_t qo_tok, int64_t qo_head, const void* k,
+                         int64_t k_tok, int64_t k_head, void* k_out, int64_t ko_tok, int64_t ko_head, int32_t dtype, int64_t n_tokens,
+                         int32_t n_q_heads, int32_t n_k_heads, int32_t head_dim, int32_t rotary_dim, const void* positions,
+                         int32_t positions_i64, const double* inv_freq, const void* q_weight, const void* k_weight, int32_t weight_dtype,
+                         float eps, int32_t interleaved, void* stream);
+
+/* A paged key-value cache: k_cache, v_cache [n_pages][n_heads][page_size][head_dim] of cache_dtype (BH_F16, BH_BF16, BH_I8, BH_E4M3), for the 8-bit types
+ * k_scale, v_scale [n_pages][n_heads][page_size] fp32.  Slot = page * page_size + offset; page_size: a power of two, 8..1024.
+ * int8: scale = max(fp32(amax / 127), 2^-126), code = the exact quotient x / scale, rounded to nearest even.  e4m3 (OCP, largest 448): scale
+ * = the least power of two >= 2^-126 with amax <= 448 * scale, code = x / scale rounded to nearest even.  A vector that holds an infinity or a NaN: scale = NaN, codes 0.
+ * bh_op_kv_write: rows k, v [n_tokens][n_heads][head_dim] of dtype (fp16, bf16, fp32) go to their slots; a slot outside
+ * [0, n_pages * page_size) is skipped.  Slots of one call must differ (of two rows with the same slot no whole vector need remain).
+ * bh_op_kv_read: the slots' vectors as dtype, code * scale rounded once; zeros for a slot outside the cache. */
+int bh_op_kv_write(const void* k, int64_t k_tok, int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, int32_t dtype,
+                   const int64_t* slots, int64_t n_tokens, int32_t n_heads, int32_t head_dim, void* k_cache, void* v_cache, float* k_scale,
+                   float* v_scale, int32_t cache_dtype, int64_t n_pages, int32_t page_size, void* stream);
+int bh_op_kv_read(void* k, int64_t k_tok, int64_t k_head, void* v, int64_t v_tok, int64_t v_head, int32_t dtype, const int64_t* slots,
+                  int64_t n_tokens, int32_t n_heads, int32_t head_dim, const void* k_cache, const void* v_cache, const float* k_scale,
+                  const float* v_scale, int32_t cache_dtype, int64_t n_pages, int32_t page_size, void* stream);
+
+/* Attention of one new token per sequence over that cache: q [batch][n_q_heads][head_dim] (fp16 or bf16; head_dim a multiple of 16, 16..256),
+ * cache_dtype = dtype, BH_I8 or BH_E4M3; query head h reads key head h / (n_q_heads / n_k_heads).  Sequence b has lengths[b] tokens in
+ * the cache (its newest among them), token t in page table[b * table_stride + t / page_size]; a length is taken as at least 0 and at
+ * most table_width * page_size, and the tokens of a table entry outside [0, n_pages) are left out.  s_t = scale q . k_t; softcap c > 0: s = c tanh(s / c); slopes (fp32 [n_q_heads] or
+ * NULL): s -= slope (length - 1 - t); window w > 0: the last w tokens only.  out [batch][n_q_heads][head_dim] of dtype; lse (fp32
+ * [batch][n_q_heads] or NULL) = log sum e^s.  Where nothing is left: out 0, lse -inf.  workspace: at least bh_op_paged_attention_workspace bytes (that returns
+ * a negative bh_status for bad sizes), 16-byte aligned. */
+int64_t bh_op_paged_attention_workspace(int32_t batch, int32_t n_q_heads, int32_t n_k_heads, int32_t head_dim, int32_t page_size,
+                                        int32_t table_width, int32_t window);
+int bh_op_paged_attention(const void* q, int64_t q_seq, int64_t q_head, int32_t dtype, const void* k_cache, const void* v_cache,
+                          const float* k_scale, const float* v_scale, int32_t cache_dtype, int64_t n_pages, int32_t page_size,
+                          const int32_t* table, int64_t table_stride, int32_t table_width, const int32_t* lengths, int32_t batch,
+                          int32_t n_q_heads, int32_t n_k_heads, int32_t head_dim, float scale, float softcap, int32_t window,
+                          const float* slopes, void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Log probabilities of given tokens, entropy and the `top` likeliest tokens (0..64) of each row of logits [n_rows][vocab] (fp16, bf16, fp32): logprobs[r][g]
+ * = log softmax(logits[r])[targets[r][g]] (0 for a negative target, NaN for one >= vocab), entropy[r] in nats, top_ids / top_logprobs
+ * [r][top] in the order (logit descending, id ascending).  -inf carries no probability; a row of nothing else has log probabilities -inf and entropy 0.  A row
+ * that holds a NaN or +inf: log probabilities and entropy NaN, alternatives in the order of its logits with NaN below -inf. */
+int64_t bh_op_token_logprobs_workspace(int64_t n_rows, int64_t vocab, int32_t dtype, int32_t top);
+int bh_op_token_logprobs(const void* logits, int64_t row_stride, int32_t dtype, int64_t n_rows, int64_t vocab, const int64_t* targets,
+                         int32_t n_given, int32_t top, float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids,
+                         void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Sparse (SPLADE) index: resident CSR corpus + exact sparse search ------------------------- */
 

@@ -1,0 +1,187 @@
+"""CPU: the decoding operators' checks of arguments (bergen_amd/decoding.py and the C entry points), which come before anything
+touches a device, and the checker's own formulas against differences it does not share."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import bergen_amd
+import decoding_reference as ref
+from bergen_amd import _lib
+
+P = ctypes.c_void_p(4096)  # an address that no refused call reads
+
+
+def _refused(match, fn, *a, **k):
+    with pytest.raises(ValueError, match=match):
+        fn(*a, **k)
+
+
+def _rotary_args(t=3, hq=4, hk=2, d=64, r=64, dtype=torch.bfloat16):
+    return dict(q=torch.zeros(t, hq, d, dtype=dtype), k=torch.zeros(t, hk, d, dtype=dtype), positions=torch.zeros(t, dtype=torch.int64),
+                inv_freq=torch.zeros(r // 2, dtype=torch.float64))
+
+
+@pytest.mark.parametrize("change, match", [
+    (dict(q=torch.zeros(3, 4, dtype=torch.bfloat16)), r"q must be \[tokens, heads, dim\]"),
+    (dict(q=torch.zeros(3, 4, 64, dtype=torch.float64)), "float16, bfloat16 or float32"),
+    (dict(k=torch.zeros(3, 2, 32, dtype=torch.bfloat16)), "k has shape"),
+    (dict(k=torch.zeros(2, 2, 64, dtype=torch.bfloat16)), "k must be"),
+    (dict(k=torch.zeros(3, 2, 64, dtype=torch.float16)), "k must be"),
+    (dict(positions=torch.zeros(3)), "positions"),
+    (dict(positions=torch.zeros(4, dtype=torch.int64)), "positions"),
+    (dict(inv_freq=torch.zeros(32)), "inv_freq must be float64"),
+    (dict(inv_freq=torch.zeros(33, dtype=torch.float64)), "rotary_dim at most 64"),
+    (dict(q_weight=torch.zeros(32, dtype=torch.bfloat16)), "q_weight"),
+    (dict(q_weight=torch.zeros(64, dtype=torch.float16)), "q_weight"),
+    (dict(q_weight=torch.zeros(64), k_weight=torch.zeros(64, dtype=torch.bfloat16)), "one type"),
+    (dict(q=torch.zeros(3, 4, 128, dtype=torch.bfloat16)[..., ::2]), "dense"),
+    (dict(q=torch.zeros(1, 4, 64, dtype=torch.bfloat16).expand(3, 4, 64), inplace=True), "overlaps itself"),
+    (dict(), "must be on the GPU"),
+])
+def test_rotary_refusals(change, match):
+    _refused(match, bergen_amd.qk_norm_rotary, **{**_rotary_args(), **change})
+
+
+def _cache_args(dtype=torch.int8, pages=2, heads=3, page=16, dim=32):
+    c = bergen_amd.kv_cache(pages, heads, page, dim, dtype, device="cpu")
+    return dict(k_cache=c.k_cache, v_cache=c.v_cache, k_scale=c.k_scale, v_scale=c.v_scale)
+
+
+def test_cache_refusals():
+    k = torch.zeros(5, 3, 32)
+    slots = torch.zeros(5, dtype=torch.int64)
+    base = dict(k=k, v=k, slots=slots, **_cache_args())
+    for change, match in [(dict(k=torch.zeros(5, 2, 32)), "k has shape"), (dict(v=torch.zeros(4, 3, 32)), "v must have"),
+                          (dict(v=k.half()), "v must have"), (dict(slots=slots.int()), "slots"), (dict(slots=slots[:4]), "slots"),
+                          (dict(k_scale=None), "needs k_scale"), (dict(v_scale=torch.zeros(2, 3, 16).double()), "needs v_scale"),
+                          (dict(v_cache=torch.zeros(2, 3, 16, 32)), "v_cache must have"),
+                          (dict(k_cache=torch.zeros(2, 3, 16, 32), v_cache=torch.zeros(2, 3, 16, 32)), "k_cache must be"),
+                          (dict(k_cache=base["k_cache"].transpose(0, 1), v_cache=base["v_cache"].transpose(0, 1)), "contiguous"),
+                          (dict(), "must be on the GPU")]:
+        _refused(match, bergen_amd.kv_cache_write, **{**base, **change})
+    half = dict(_cache_args(torch.float16), k_scale=torch.zeros(2, 3, 16))
+    _refused("has no scales", bergen_amd.kv_cache_read, slots, **half)
+    _refused("dtype must be", bergen_amd.kv_cache_read, slots, **_cache_args(), dtype=torch.int8)
+    _refused("must be on the GPU", bergen_amd.kv_cache_read, slots, **_cache_args())
+    _refused("a cache holds", bergen_amd.kv_cache, 1, 1, 16, 32, torch.float32, device="cpu")
+
+
+def test_attention_refusals():
+    base = dict(q=torch.zeros(2, 6, 32, dtype=torch.bfloat16), block_table=torch.zeros(2, 4, dtype=torch.int32),
+                lengths=torch.zeros(2, dtype=torch.int32), **_cache_args())
+    for change, match in [(dict(q=torch.zeros(2, 6, 32)), "q must be float16 or bfloat16"), (dict(q=torch.zeros(2, 6, 48, dtype=torch.bfloat16)), "q has shape"),
+                          (dict(block_table=torch.zeros(3, 4, dtype=torch.int32)), "block_table"), (dict(block_table=torch.zeros(2, 4).long()), "block_table"),
+                          (dict(lengths=torch.zeros(2)), "lengths"), (dict(lengths=torch.zeros(3, dtype=torch.int32)), "lengths"),
+                          (dict(alibi_slopes=torch.zeros(3)), "alibi_slopes"), (_cache_args(torch.float16), "the cache must be"),
+                          (dict(), "must be on the GPU")]:
+        _refused(match, bergen_amd.paged_attention, **{**base, **change})
+
+
+def test_logprobs_refusals():
+    x, t = torch.zeros(2, 9), torch.zeros(2, dtype=torch.int64)
+    for a, match in [((x.double(), t), "logits must be"), ((x[0], t), "logits must be"), ((x[:, :0], t), "not empty"), ((x.t(), t), "dense"),
+                     ((x, t.int()), "targets"), ((x, t[:1]), "targets"), ((x, t), "must be on the GPU")]:
+        _refused(match, bergen_amd.token_logprobs, *a)
+
+
+def test_refused_by_the_c_entry_points():
+    """Sizes, types, null buffers and short workspaces are refused before any device is looked for, each with its message."""
+    lib, E, U = _lib.lib(), _lib.BH_EINVAL, _lib.BH_EUNSUPPORTED
+    H, B, F, I8, E4 = _lib.BH_F16, _lib.BH_BF16, _lib.BH_F32, _lib.BH_I8, _lib.BH_E4M3
+
+    def rotary(dtype=B, tokens=2, nq=2, nk=1, dim=64, rot=64, pos=P, inv=P, qw=None, wt=B, eps=1e-6, q=P):
+        return lib.bh_op_qk_norm_rotary(q, 128, 64, P, 128, 64, P, 64, 64, P, 64, 64, dtype, tokens, nq, nk, dim, rot, pos, 1, inv, qw, None, wt, eps, 0, None)
+
+    for code, k in [(E, dict(dtype=I8)), (E, dict(dtype=9)), (E, dict(qw=P, wt=H)), (E, dict(tokens=-1)), (E, dict(nq=0)), (E, dict(eps=-1.0)),
+                    (E, dict(eps=math.nan)), (U, dict(dim=257)), (U, dict(dim=0)), (E, dict(rot=66)), (E, dict(rot=63)), (E, dict(rot=-2)),
+                    (U, dict(tokens=1 << 31)), (E, dict(q=None)), (E, dict(pos=None)), (E, dict(inv=None))]:
+        assert rotary(**k) == code, k
+        assert lib.bh_last_error(), k
+    assert rotary(tokens=0) == _lib.BH_OK
+
+    def write(dtype=B, cache=I8, tokens=2, heads=2, dim=64, pages=4, page=16, k=P, slots=P, scale=P, fn=lib.bh_op_kv_write):
+        return fn(k, 128, 64, P, 128, 64, dtype, slots, tokens, heads, dim, P, P, scale, scale, cache, pages, page, None)
+
+    for fn in (lib.bh_op_kv_write, lib.bh_op_kv_read):
+        for code, k in [(E, dict(dtype=I8)), (E, dict(cache=F)), (E, dict(cache=7)), (E, dict(tokens=-1)), (E, dict(heads=0)), (E, dict(pages=0)),
+                        (U, dict(dim=257)), (U, dict(page=4)), (U, dict(page=24)), (U, dict(page=2048)), (E, dict(k=None)), (E, dict(slots=None)),
+                        (E, dict(scale=None)), (U, dict(tokens=1 << 40)), (U, dict(tokens=1 << 28))]:
+            assert write(fn=fn, **k) == code, k
+        assert write(fn=fn, tokens=0) == _lib.BH_OK
+
+    def attend(dtype=B, cache=B, batch=2, hq=8, hk=2, dim=64, page=16, width=4, q=P, kc=P, scale=None, s=0.125, cap=0.0, window=0, ws=P, n=1 << 40, pages=9,
+               q_seq=512):
+        return lib.bh_op_paged_attention(q, q_seq, 64, dtype, kc, P, scale, scale, cache, pages, page, P, width, width, P, batch, hq, hk, dim, s, cap,
+                                         window, None, P, None, ws, n, None)
+
+    for code, k in [(E, dict(dtype=F)), (E, dict(cache=H)), (E, dict(cache=F)), (E, dict(batch=-1)), (E, dict(hq=7)), (E, dict(hk=0)), (U, dict(dim=72)),
+                    (U, dict(dim=272)), (U, dict(page=4)), (U, dict(page=48)), (E, dict(width=-1)), (U, dict(batch=65536)), (U, dict(width=1 << 30)),
+                    (E, dict(s=math.nan)), (E, dict(cap=-1.0)), (E, dict(cap=math.inf)), (E, dict(cap=math.nan)), (E, dict(window=-1)), (E, dict(q=None)),
+                    (E, dict(kc=None)), (E, dict(cache=E4)), (E, dict(pages=-1)), (U, dict(q=ctypes.c_void_p(4098))), (U, dict(q_seq=511)),
+                    (E, dict(width=4096, n=1024)), (E, dict(width=4096, ws=None)), (E, dict(width=4096, ws=ctypes.c_void_p(4104)))]:
+        assert attend(**k) == code, k
+        assert lib.bh_last_error(), k
+    assert attend(batch=0) == _lib.BH_OK
+    size = lib.bh_op_paged_attention_workspace
+    assert size(2, 8, 2, 64, 16, 4096, 0) > 0 and size(0, 8, 2, 64, 16, 4096, 0) == 0
+    assert size(2, 7, 2, 64, 16, 4, 0) == E and size(2, 8, 2, 60, 16, 4, 0) == U and size(2, 8, 2, 64, 16, 4, -1) == E
+
+    def logp(dtype=F, rows=2, vocab=100, given=1, top=5, x=P, t=P, ids=P, ws=P, n=1 << 40, stride=100):
+        return lib.bh_op_token_logprobs(x, stride, dtype, rows, vocab, t, given, top, P, P, P, ids, ws, n, None)
+
+    for code, k in [(E, dict(dtype=I8)), (E, dict(rows=-1)), (E, dict(vocab=0)), (E, dict(top=101)), (E, dict(top=-1)), (U, dict(top=65)), (E, dict(given=-1)),
+                    (E, dict(stride=99)), (E, dict(x=None)), (E, dict(t=None)), (E, dict(ids=None)), (U, dict(vocab=(1 << 30) + 1, stride=1 << 31)),
+                    (U, dict(rows=(1 << 24) + 1)), (E, dict(x=ctypes.c_void_p(4098))), (E, dict(vocab=100000, stride=100000, n=8)),
+                    (E, dict(vocab=100000, stride=100000, ws=None))]:
+        assert logp(**k) == code, k
+    assert logp(rows=0) == _lib.BH_OK
+    assert lib.bh_op_token_logprobs_workspace(1, 100000, F, 5) > 0 and lib.bh_op_token_logprobs_workspace(100000, 1000, F, 5) == 0
+    assert lib.bh_op_token_logprobs_workspace(1, 100, F, 101) == E
+
+
+def test_older_entry_points_still_refuse_the_new_types():
+    lib = _lib.lib()
+    h = ctypes.c_void_p()
+    for t in (_lib.BH_BF16, _lib.BH_I8, _lib.BH_E4M3):
+        assert lib.bh_index_create(ctypes.byref(h), 10, 64, t, 0) in (_lib.BH_EINVAL, _lib.BH_EUNSUPPORTED)
+
+
+def test_a_gradient_is_refused_while_it_is_recorded():
+    from bergen_amd import decoding
+
+    class OnGpu:  # what the check looks at, without a device
+        requires_grad, device = True, torch.device("cuda", 0)
+    with pytest.raises(ValueError, match="no backward pass"):
+        decoding._same_device(OnGpu())
+
+
+def test_rotary_frequencies():
+    f = bergen_amd.rotary_frequencies(8, 100.0, 0.5, device="cpu")
+    assert f.dtype == torch.float64 and torch.allclose(f, 0.5 * torch.tensor([1, 100 ** -0.25, 0.1, 100 ** -0.75], dtype=torch.float64), rtol=1e-15)
+    assert bergen_amd.rotary_frequencies(0, device="cpu").numel() == 0
+    _refused("even", bergen_amd.rotary_frequencies, 7, device="cpu")
+
+
+def test_the_checker_against_torch():
+    """The 64-bit checkers agree with torch's own functions where torch has one."""
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(5, 301, generator=g)
+    r = ref.logprobs(x, torch.arange(5), 7)
+    lp = torch.log_softmax(x.double(), -1)
+    assert torch.allclose(r["logprobs"][0], lp[torch.arange(5), torch.arange(5)], atol=1e-12)
+    assert torch.allclose(r["entropy"][0], torch.distributions.Categorical(logits=x.double()).entropy(), atol=1e-12)
+    assert torch.equal(r["top_ids"], x.topk(7).indices)
+    y = torch.randn(1000, generator=g) * 200
+    codes, scale = ref.quantise(y[None], torch.float8_e4m3fn)
+    assert torch.equal(codes[0], (y / scale).to(torch.float8_e4m3fn).double()) and 224 < float(y.abs().max() / scale) <= 448
+    codes, scale = ref.quantise(y[None], torch.int8)
+    assert float(codes.abs().max()) == 127
+    c = bergen_amd.kv_cache(3, 2, 8, 16, torch.float16, device="cpu")
+    c.k_cache.normal_(generator=g), c.v_cache.normal_(generator=g)
+    q = torch.randn(1, 4, 16, generator=g).half()
+    out, _, lse, _ = ref.attention(q, c.k_cache, c.v_cache, torch.tensor([[2, 0]], dtype=torch.int32), torch.tensor([13]))
+    k, v = (torch.cat([z[2], z[0]], 1)[:, :13].double().repeat_interleave(2, 0) for z in (c.k_cache, c.v_cache))
+    want = torch.nn.functional.scaled_dot_product_attention(q[0].double()[:, None], k, v)[:, 0]
+    assert torch.allclose(out[0], want, atol=1e-12)
