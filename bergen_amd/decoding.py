@@ -29,22 +29,28 @@ TokenLogprobs = collections.namedtuple("TokenLogprobs", "logprobs entropy top_lo
 
 _ready = set()
 
+# the current stream's handle: current_stream() builds an object around it, which takes longer than the launch it is wanted for
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
-def _need(ok, message):
-    if not ok:
-        raise ValueError(message)
+
+def _fail(message):
+    raise ValueError(message)
 
 
 def _same_device(first, **others):
     """Every tensor on one GPU, and none that waits for a gradient; -> that device."""
     device = first.device
-    _need(device.type == "cuda", f"tensors must be on the GPU, got one on {device}")
+    if device.type != "cuda":
+        _fail(f"tensors must be on the GPU, got one on {device}")
     grad = torch.is_grad_enabled()
-    _need(not (grad and first.requires_grad), "no backward pass here: call under torch.no_grad()")
+    if grad and first.requires_grad:
+        _fail("no backward pass here: call under torch.no_grad()")
     for name, t in others.items():
         if t is not None:
-            _need(t.device == device, f"{name} is on {t.device}, expected {device}")
-            _need(not (grad and t.requires_grad), f"{name} requires a gradient and there is no backward pass here: call under torch.no_grad()")
+            if t.device != device:
+                _fail(f"{name} is on {t.device}, expected {device}")
+            if grad and t.requires_grad:
+                _fail(f"{name} requires a gradient and there is no backward pass here: call under torch.no_grad()")
     if device.index not in _ready:
         with torch.cuda.device(device):
             _lib.init(device.index)  # once per device: is it a gfx950 part
@@ -54,7 +60,7 @@ def _same_device(first, **others):
 
 def _call(device, fn, *args):
     """fn(*args, stream) with the tensors' device as the current one, on its current stream."""
-    stream = torch.cuda.current_stream(device).cuda_stream
+    stream = _stream(device.index)
     if torch.cuda.current_device() == device.index:
         _lib.check(fn(*args, stream))
     else:
@@ -64,10 +70,14 @@ def _call(device, fn, *args):
 
 def _rows(name, t, heads=None, dim=None):
     """[tokens, heads, dim] with the last dimension dense."""
-    _need(t.dim() == 3, f"{name} must be [tokens, heads, dim], got {tuple(t.shape)}")
-    _need(t.dtype in _FLOATS, f"{name} must be float16, bfloat16 or float32, got {t.dtype}")
-    _need((heads is None or t.shape[1] == heads) and (dim is None or t.shape[2] == dim), f"{name} has shape {tuple(t.shape)}")
-    _need(t.shape[2] <= 1 or t.stride(2) == 1, f"{name}'s last dimension must be dense")
+    if t.dim() != 3:
+        _fail(f"{name} must be [tokens, heads, dim], got {tuple(t.shape)}")
+    if t.dtype not in _FLOATS:
+        _fail(f"{name} must be float16, bfloat16 or float32, got {t.dtype}")
+    if not ((heads is None or t.shape[1] == heads) and (dim is None or t.shape[2] == dim)):
+        _fail(f"{name} has shape {tuple(t.shape)}")
+    if not (t.shape[2] <= 1 or t.stride(2) == 1):
+        _fail(f"{name}'s last dimension must be dense")
 
 
 def _distinct(name, t):
@@ -75,13 +85,32 @@ def _distinct(name, t):
     room = 1
     for size, stride in sorted(zip(t.shape, t.stride()), key=lambda p: p[1]):
         if size > 1:
-            _need(stride >= room, f"{name} overlaps itself (shape {tuple(t.shape)}, strides {t.stride()}): it cannot be written")
+            if not (stride >= room):
+                _fail(f"{name} overlaps itself (shape {tuple(t.shape)}, strides {t.stride()}): it cannot be written")
             room = stride * size
+
+
+def _apart(q, k):
+    """q's and k's memory does not meet: separate ranges, or separate columns of rows that are equally far apart."""
+    size = q.element_size()
+    if 0 in q.shape or 0 in k.shape:
+        return
+    ends = [sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1 for t in (q, k)]
+    at = (k.data_ptr() - q.data_ptr()) // size
+    if at >= ends[0] or -at >= ends[1]:
+        return
+    row = q.stride(0)
+    if q.shape[0] > 1 and k.stride(0) == row:
+        cols = [e - (t.shape[0] - 1) * row for e, t in zip(ends, (q, k))]
+        if at % row >= cols[0] and at % row + cols[1] <= row:
+            return
+    _fail("q and k overlap: they cannot be written in place")
 
 
 def rotary_frequencies(rotary_dim, theta=10000.0, scale=1.0, device="cuda"):
     """inv_freq[j] = scale * theta^(-2 j / rotary_dim), j < rotary_dim / 2, float64: what `qk_norm_rotary` turns a pair by, per position."""
-    _need(rotary_dim >= 0 and rotary_dim % 2 == 0, f"rotary_dim must be even, got {rotary_dim}")
+    if not (rotary_dim >= 0 and rotary_dim % 2 == 0):
+        _fail(f"rotary_dim must be even, got {rotary_dim}")
     j = torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device)
     return float(scale) * float(theta) ** (-j / max(1, rotary_dim))
 
@@ -97,23 +126,30 @@ def qk_norm_rotary(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=
     _rows("q", q)
     _rows("k", k, dim=q.shape[2])
     tokens, nq, dim = q.shape
-    _need(k.dtype == q.dtype and k.shape[0] == tokens, f"k must be [{tokens}, heads, {dim}] {q.dtype}, got {tuple(k.shape)} {k.dtype}")
-    _need(positions.shape == (tokens,) and positions.dtype in (torch.int32, torch.int64), f"positions must be int32 or int64 [{tokens}]")
-    _need(inv_freq.dim() == 1 and inv_freq.dtype == torch.float64 and 2 * inv_freq.numel() <= dim,
-          f"inv_freq must be float64 [rotary_dim / 2], rotary_dim at most {dim}")
+    if not (k.dtype == q.dtype and k.shape[0] == tokens):
+        _fail(f"k must be [{tokens}, heads, {dim}] {q.dtype}, got {tuple(k.shape)} {k.dtype}")
+    if not (positions.shape == (tokens,) and positions.dtype in (torch.int32, torch.int64)):
+        _fail(f"positions must be int32 or int64 [{tokens}]")
+    if not (inv_freq.dim() == 1 and inv_freq.dtype == torch.float64 and 2 * inv_freq.numel() <= dim):
+        _fail(f"inv_freq must be float64 [rotary_dim / 2], rotary_dim at most {dim}")
     wtype = None
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w is not None:
-            _need(w.shape == (dim,) and w.dtype in (q.dtype, torch.float32), f"{name} must be [{dim}], {q.dtype} or float32")
-            _need(wtype in (None, w.dtype), "q_weight and k_weight must have one type")
-            _need(w.is_contiguous(), f"{name} must be contiguous")
+            if not (w.shape == (dim,) and w.dtype in (q.dtype, torch.float32)):
+                _fail(f"{name} must be [{dim}], {q.dtype} or float32")
+            if not (wtype in (None, w.dtype)):
+                _fail("q_weight and k_weight must have one type")
+            if not w.is_contiguous():
+                _fail(f"{name} must be contiguous")
             wtype = w.dtype
-    _need(positions.is_contiguous() and inv_freq.is_contiguous(), "positions and inv_freq must be contiguous")
+    if not (positions.is_contiguous() and inv_freq.is_contiguous()):
+        _fail("positions and inv_freq must be contiguous")
     if inplace:
         _distinct("q", q)
         _distinct("k", k)
+        _apart(q, k)
     device = _same_device(q, k=k, positions=positions, inv_freq=inv_freq, q_weight=q_weight, k_weight=k_weight)
-    qo, ko = (q, k) if inplace else (torch.empty(q.shape, dtype=q.dtype, device=device), torch.empty(k.shape, dtype=k.dtype, device=device))
+    qo, ko = (q, k) if inplace else (q.new_empty(q.shape), k.new_empty(k.shape))
     _call(device, _lib.lib().bh_op_qk_norm_rotary, q.data_ptr(), q.stride(0), q.stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1),
           k.data_ptr(), k.stride(0), k.stride(1), ko.data_ptr(), ko.stride(0), ko.stride(1), _FLOATS[q.dtype], tokens, nq, k.shape[1], dim,
           2 * inv_freq.numel(), positions.data_ptr(), int(positions.dtype == torch.int64), inv_freq.data_ptr(),
@@ -127,7 +163,8 @@ KVCache = collections.namedtuple("KVCache", "k_cache v_cache k_scale v_scale")
 
 def kv_cache(pages, heads, page_size, dim, dtype=torch.bfloat16, device="cuda"):
     """An empty paged cache -> KVCache(k_cache, v_cache [pages, heads, page_size, dim], k_scale, v_scale [pages, heads, page_size] or None)."""
-    _need(dtype in _CACHES, f"a cache holds float16, bfloat16, int8 or float8_e4m3fn, got {dtype}")
+    if not (dtype in _CACHES):
+        _fail(f"a cache holds float16, bfloat16, int8 or float8_e4m3fn, got {dtype}")
     shape = (pages, heads, page_size, dim)
     made = [torch.zeros(shape, dtype=torch.int8 if dtype in _SCALED else dtype, device=device).view(dtype) for _ in range(2)]
     scales = [torch.zeros(shape[:3], dtype=torch.float32, device=device) if dtype in _SCALED else None for _ in range(2)]
@@ -135,16 +172,19 @@ def kv_cache(pages, heads, page_size, dim, dtype=torch.bfloat16, device="cuda"):
 
 
 def _cache_tensors(k_cache, v_cache, k_scale, v_scale):
-    _need(k_cache.dim() == 4 and k_cache.dtype in _CACHES, f"k_cache must be [pages, heads, page_size, dim], float16, bfloat16, int8 or float8_e4m3fn; "
-          f"got {tuple(k_cache.shape)} {k_cache.dtype}")
-    _need(v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype, "v_cache must have k_cache's shape and type")
-    _need(k_cache.is_contiguous() and v_cache.is_contiguous(), "k_cache and v_cache must be contiguous")
+    if not (k_cache.dim() == 4 and k_cache.dtype in _CACHES):
+        _fail(f"k_cache must be [pages, heads, page_size, dim], float16, bfloat16, int8 or float8_e4m3fn; " f"got {tuple(k_cache.shape)} {k_cache.dtype}")
+    if not (v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype):
+        _fail("v_cache must have k_cache's shape and type")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        _fail("k_cache and v_cache must be contiguous")
     if k_cache.dtype in _SCALED:
         for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
-            _need(s is not None and s.shape == k_cache.shape[:3] and s.dtype == torch.float32 and s.is_contiguous(),
-                  f"an 8-bit cache needs {name}: contiguous float32 {tuple(k_cache.shape[:3])}")
+            if not (s is not None and s.shape == k_cache.shape[:3] and s.dtype == torch.float32 and s.is_contiguous()):
+                _fail(f"an 8-bit cache needs {name}: contiguous float32 {tuple(k_cache.shape[:3])}")
     else:
-        _need(k_scale is None and v_scale is None, f"a cache of {k_cache.dtype} has no scales")
+        if not (k_scale is None and v_scale is None):
+            _fail(f"a cache of {k_cache.dtype} has no scales")
 
 
 def _ptr(t):
@@ -162,8 +202,10 @@ def kv_cache_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
     pages, heads, page, dim = k_cache.shape
     _rows("k", k, heads, dim)
     _rows("v", v, heads, dim)
-    _need(v.shape == k.shape and v.dtype == k.dtype, "v must have k's shape and type")
-    _need(slots.shape == (k.shape[0],) and slots.dtype == torch.int64 and slots.is_contiguous(), f"slots must be contiguous int64 [{k.shape[0]}]")
+    if not (v.shape == k.shape and v.dtype == k.dtype):
+        _fail("v must have k's shape and type")
+    if not (slots.shape == (k.shape[0],) and slots.dtype == torch.int64 and slots.is_contiguous()):
+        _fail(f"slots must be contiguous int64 [{k.shape[0]}]")
     device = _same_device(k, v=v, slots=slots, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale)
     _call(device, _lib.lib().bh_op_kv_write, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _FLOATS[k.dtype],
           slots.data_ptr(), k.shape[0], heads, dim, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), _CACHES[k_cache.dtype],
@@ -174,8 +216,10 @@ def kv_cache_read(slots, k_cache, v_cache, k_scale=None, v_scale=None, dtype=tor
     """The slots' keys and values (int64 [tokens]) as `dtype` -> (k, v) [tokens, heads, dim]; zeros for a slot outside the cache."""
     _cache_tensors(k_cache, v_cache, k_scale, v_scale)
     pages, heads, page, dim = k_cache.shape
-    _need(dtype in _FLOATS, f"dtype must be float16, bfloat16 or float32, got {dtype}")
-    _need(slots.dim() == 1 and slots.dtype == torch.int64 and slots.is_contiguous(), "slots must be contiguous int64 [tokens]")
+    if not (dtype in _FLOATS):
+        _fail(f"dtype must be float16, bfloat16 or float32, got {dtype}")
+    if not (slots.dim() == 1 and slots.dtype == torch.int64 and slots.is_contiguous()):
+        _fail("slots must be contiguous int64 [tokens]")
     device = _same_device(slots, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale)
     k, v = (torch.empty((slots.shape[0], heads, dim), dtype=dtype, device=device) for _ in range(2))
     _call(device, _lib.lib().bh_op_kv_read, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _FLOATS[dtype],
@@ -199,14 +243,17 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, scale=None, k_sca
     pages, heads, page, dim = k_cache.shape
     _rows("q", q, dim=dim)
     batch, nq, _ = q.shape
-    _need(q.dtype in (torch.float16, torch.bfloat16), f"q must be float16 or bfloat16, got {q.dtype}")
-    _need(k_cache.dtype == q.dtype or k_cache.dtype in _SCALED, f"the cache must be {q.dtype}, int8 or float8_e4m3fn, got {k_cache.dtype}")
-    _need(block_table.dim() == 2 and block_table.shape[0] == batch and block_table.dtype == torch.int32
-          and (block_table.shape[1] <= 1 or block_table.stride(1) == 1), f"block_table must be int32 [{batch}, width] with dense rows")
-    _need(lengths.shape == (batch,) and lengths.dtype == torch.int32 and lengths.is_contiguous(), f"lengths must be contiguous int32 [{batch}]")
+    if not (q.dtype in (torch.float16, torch.bfloat16)):
+        _fail(f"q must be float16 or bfloat16, got {q.dtype}")
+    if not (k_cache.dtype == q.dtype or k_cache.dtype in _SCALED):
+        _fail(f"the cache must be {q.dtype}, int8 or float8_e4m3fn, got {k_cache.dtype}")
+    if not (block_table.dim() == 2 and block_table.shape[0] == batch and block_table.dtype == torch.int32 and (block_table.shape[1] <= 1 or block_table.stride(1) == 1)):
+        _fail(f"block_table must be int32 [{batch}, width] with dense rows")
+    if not (lengths.shape == (batch,) and lengths.dtype == torch.int32 and lengths.is_contiguous()):
+        _fail(f"lengths must be contiguous int32 [{batch}]")
     if alibi_slopes is not None:
-        _need(alibi_slopes.shape == (nq,) and alibi_slopes.dtype == torch.float32 and alibi_slopes.is_contiguous(),
-              f"alibi_slopes must be contiguous float32 [{nq}]")
+        if not (alibi_slopes.shape == (nq,) and alibi_slopes.dtype == torch.float32 and alibi_slopes.is_contiguous()):
+            _fail(f"alibi_slopes must be contiguous float32 [{nq}]")
     device = _same_device(q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, lengths=lengths, k_scale=k_scale, v_scale=v_scale,
                           alibi_slopes=alibi_slopes)
     if q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8:
@@ -215,7 +262,7 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, scale=None, k_sca
     need = lib.bh_op_paged_attention_workspace(batch, nq, heads, dim, page, width, int(window))
     if need < 0:
         _lib.check(need)
-    out = torch.empty((batch, nq, dim), dtype=q.dtype, device=device)
+    out = q.new_empty((batch, nq, dim))
     lse = torch.empty((batch, nq), dtype=torch.float32, device=device) if return_lse else None
     # (made anew for each call: two calls at once, or two captured graphs, must not share one)
     work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
@@ -234,11 +281,13 @@ def token_logprobs(logits, targets, top=0):
     A negative target's log probability is 0 (padding), one beyond the vocabulary NaN.  -inf logits carry no probability; a row of nothing
     else has log probabilities -inf and entropy 0; a row with a NaN or +inf has NaN.  top is at most 64.
     """
-    _need(logits.dim() == 2 and logits.dtype in _FLOATS, f"logits must be [rows, vocab], float16, bfloat16 or float32; got {tuple(logits.shape)} {logits.dtype}")
+    if not (logits.dim() == 2 and logits.dtype in _FLOATS):
+        _fail(f"logits must be [rows, vocab], float16, bfloat16 or float32; got {tuple(logits.shape)} {logits.dtype}")
     rows, vocab = logits.shape
-    _need(vocab >= 1 and (vocab == 1 or logits.stride(1) == 1), "logits' rows must be dense and not empty")
-    _need(targets.dtype == torch.int64 and targets.dim() in (1, 2) and targets.shape[0] == rows and targets.is_contiguous(),
-          f"targets must be contiguous int64 [{rows}] or [{rows}, given]")
+    if not (vocab >= 1 and (vocab == 1 or logits.stride(1) == 1)):
+        _fail("logits' rows must be dense and not empty")
+    if not (targets.dtype == torch.int64 and targets.dim() in (1, 2) and targets.shape[0] == rows and targets.is_contiguous()):
+        _fail(f"targets must be contiguous int64 [{rows}] or [{rows}, given]")
     device = _same_device(logits, targets=targets)
     if rows > 1 and logits.stride(0) < vocab:
         logits = logits.contiguous()
@@ -246,10 +295,10 @@ def token_logprobs(logits, targets, top=0):
     need = lib.bh_op_token_logprobs_workspace(rows, vocab, _FLOATS[logits.dtype], top)
     if need < 0:
         _lib.check(need)
-    logprobs = torch.empty(targets.shape, dtype=torch.float32, device=device)
-    entropy = torch.empty((rows,), dtype=torch.float32, device=device)
-    top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=device)
-    top_ids = torch.empty((rows, top), dtype=torch.int64, device=device)
+    logprobs = logits.new_empty(targets.shape, dtype=torch.float32)
+    entropy = logits.new_empty((rows,), dtype=torch.float32)
+    top_logprobs = logits.new_empty((rows, top), dtype=torch.float32)
+    top_ids = targets.new_empty((rows, top))
     work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _call(device, lib.bh_op_token_logprobs, logits.data_ptr(), logits.stride(0), _FLOATS[logits.dtype], rows, vocab, targets.data_ptr(),
           1 if targets.dim() == 1 else targets.shape[1], top, logprobs.data_ptr(), entropy.data_ptr(), top_logprobs.data_ptr(),

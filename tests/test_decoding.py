@@ -23,6 +23,9 @@ def _rotary_args(t=3, hq=4, hk=2, d=64, r=64, dtype=torch.bfloat16):
                 inv_freq=torch.zeros(r // 2, dtype=torch.float64))
 
 
+_QKV = torch.zeros(3, 8, 64, dtype=torch.bfloat16)
+
+
 @pytest.mark.parametrize("change, match", [
     (dict(q=torch.zeros(3, 4, dtype=torch.bfloat16)), r"q must be \[tokens, heads, dim\]"),
     (dict(q=torch.zeros(3, 4, 64, dtype=torch.float64)), "float16, bfloat16 or float32"),
@@ -38,6 +41,12 @@ def _rotary_args(t=3, hq=4, hk=2, d=64, r=64, dtype=torch.bfloat16):
     (dict(q_weight=torch.zeros(64), k_weight=torch.zeros(64, dtype=torch.bfloat16)), "one type"),
     (dict(q=torch.zeros(3, 4, 128, dtype=torch.bfloat16)[..., ::2]), "dense"),
     (dict(q=torch.zeros(1, 4, 64, dtype=torch.bfloat16).expand(3, 4, 64), inplace=True), "overlaps itself"),
+    (dict(q=_QKV[:, :4], k=_QKV[:, 3:5], inplace=True), "q and k overlap"),
+    (dict(q=_QKV[:, :4], k=_QKV[:, :4], inplace=True), "q and k overlap"),
+    (dict(q=_QKV[:1, :4], k=_QKV[:1, 3:], positions=torch.zeros(1, dtype=torch.int64), inplace=True), "q and k overlap"),
+    (dict(q=_QKV[:, :4], k=_QKV[:, 4:6], inplace=True), "must be on the GPU"),
+    (dict(q=_QKV[:1, :4], k=_QKV[:1, 4:], positions=torch.zeros(1, dtype=torch.int64), inplace=True), "must be on the GPU"),
+    (dict(q=_QKV[:, :4].clone(), k=_QKV[:, :4], inplace=True), "must be on the GPU"),
     (dict(), "must be on the GPU"),
 ])
 def test_rotary_refusals(change, match):
