@@ -62,6 +62,14 @@ struct Mma<__bf16> {
     static __device__ __forceinline__ floatx4 mul(frag a, frag b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 
+// A load of what is not read again: the lines need not stay (bf16 cache of 1.08 GB, 64 sequences: 186 us, 201 us with plain loads).
+// Not for 8-bit keys wider than 64 bytes, whose lines two instructions share: those were fetched twice (0.73 GB: 148 and 145 us).
+template <typename T>
+__device__ __forceinline__ T streamed(const unsigned char* p) {
+    typedef unsigned words __attribute__((ext_vector_type(sizeof(T) / 4)));
+    return __builtin_bit_cast(T, __builtin_nontemporal_load(reinterpret_cast<const words*>(p)));
+}
+
 __device__ __forceinline__ float over_groups_max(float v) {  // over the 4 lanes with the same lane % 16
     v = fmaxf(v, __shfl_xor(v, 16));
     return fmaxf(v, __shfl_xor(v, 32));
@@ -86,9 +94,10 @@ __device__ __forceinline__ unsigned two_f16(unsigned word, int which) {
                  : __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.0f, false));
 }
 
-// E: the queries' type; CACHE: BH_F16 / BH_BF16 (E's own), BH_I8, BH_E4M3; DP: head dim, rounded up to 64, 128 or 256.
-template <typename E, int CACHE, int DP>
-__global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) bh_paged_attention_kernel(PagedArgs a) {
+// E: the queries' type; CACHE: BH_F16 / BH_BF16 (E's own), BH_I8, BH_E4M3; DP: head dim, rounded up to 64, 128 or 256 (EXACT: is it).
+// ONE_PAGE: pages of 32 tokens and more, so that a tile lies in one.
+template <typename E, int CACHE, int DP, bool EXACT, bool ONE_PAGE>
+__global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : DP == 64 ? 4 : EXACT ? 3 : 2) bh_paged_attention_kernel(PagedArgs a) {
     constexpr bool SCALED = CACHE == BH_I8 || CACHE == BH_E4M3;
     typedef typename std::conditional<SCALED, _Float16, E>::type M;  // the MFMAs' type
     typedef typename Mma<M>::frag frag;
@@ -100,13 +109,16 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) bh_paged_attent
     constexpr bool F16 = std::is_same<M, _Float16>::value;
     constexpr float HOLD = F16 ? 14.f : 0.f;      // weights are held times 2^HOLD
 
+    __shared__ frag sh_q[KS][64];  // registers are short; each wave writes the same and reads what it wrote
     __shared__ float sh_stats[WAVES][2][16];
     __shared__ float sh_out[WAVES][16][DP + 4];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, n = lane & 15;
-    const int split = blockIdx.x, seq = blockIdx.z;
-    const int hk = blockIdx.y / a.blocks, block = blockIdx.y - hk * a.blocks;
+    // (splits slowest: workgroups go to the XCDs in turn, and with the splits side by side the XCDs that get every sequence's
+    // first ones would have far more to do than those that get the last ones, which most sequences do not have)
+    const int split = blockIdx.z, seq = blockIdx.y;
+    const int hk = blockIdx.x / a.blocks, block = blockIdx.x - hk * a.blocks;
     const int hq0 = hk * a.group + 16 * block;                       // the first of this workgroup's query heads
     const int heads = a.group - 16 * block < 16 ? a.group - 16 * block : 16;
 
@@ -123,7 +135,6 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) bh_paged_attent
     // ---- the queries, operand B of S^T: lane (g, n) holds head n, dims as its key chunks
     const bool head_live = n < heads;
     const E* qp = static_cast<const E*>(a.q) + seq * a.q_seq + (long long)(hq0 + (head_live ? n : 0)) * a.q_head;
-    frag qf[KS];
     float unit = a.scale * LOG2E;  // of a score, in powers of two
     {
         float top = 0.f;
@@ -136,7 +147,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) bh_paged_attent
             vec x = {};
             if (head_live && d < a.dim) x = *reinterpret_cast<const vec*>(qp + d);
             if constexpr (std::is_same<E, M>::value) {
-                qf[s] = __builtin_bit_cast(frag, x);
+                sh_q[s][lane] = __builtin_bit_cast(frag, x);
             } else {
                 qb[s] = x;
 #pragma unroll
@@ -151,30 +162,96 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) bh_paged_attent
             e = e > 126 ? 126 : e < -112 ? -112 : e;
             const float up = ldexpf(1.f, 7 - e);
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
+            for (int s = 0; s < KS; ++s) {
+                frag f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) qf[s][i] = (_Float16)((float)qb[s][i] * up);
+                for (int i = 0; i < 8; ++i) f[i] = (_Float16)((float)qb[s][i] * up);
+                sh_q[s][lane] = f;
+            }
             unit *= ldexpf(1.f, e - 7);
         }
     }
     const float slope = a.slopes && head_live ? a.slopes[hq0 + n] * LOG2E : 0.f;
+    if (DP > 64 && g == 0) sh_stats[wave][0][n] = slope;  // (kept there until the wave's own m comes; heads of 64 keep it in a register)
     const float cap = a.softcap * LOG2E, cap_unit = a.softcap > 0.f ? 2.f / a.softcap : 0.f;
 
-    float m, total;  // of head n: the same m in its 4 lanes, each lane's own sum
+    float m, total;  // of head n: the same m in its 4 lanes; each lane's own sum, times 2^HOLD
     float v_top;     // values' scales are held against a power of two
     floatx4 o[NJ];
 
     const int* table = a.table + seq * a.table_stride;
+    const int in_page = (1 << a.page_log2) - 1, last = a.table_width - 1;
+    const int row = EXACT ? DP * ES : a.dim * ES;  // bytes
+    // what a lane loads of a row: key bytes at 16 (4 s + g), value bytes at NJ ES n; behind the row's end (dim < DP) its first bytes instead
+    int key_at[KL];
+#pragma unroll
+    for (int s = 0; s < KL; ++s) key_at[s] = EXACT || 16 * (4 * s + g) < row ? 16 * (4 * s + g) : 0;
+    const int value_at = EXACT || NJ * n < a.dim ? NJ * ES * n : 0;
     const unsigned char* kc = static_cast<const unsigned char*>(a.k);
     const unsigned char* vc = static_cast<const unsigned char*>(a.v);
-    const long long row = (long long)a.dim * ES;
-    const int in_page = (1 << a.page_log2) - 1;
 
-    // the vector of token t in the cache (its index), if its page is there; t is a multiple of 8
-    auto vector_at = [&](int t, bool& there) {
-        const int page = t < len ? table[t >> a.page_log2] : -1;
-        there = page >= 0 && page < a.n_pages;
-        return ((((long long)(there ? page : 0) * a.hk + hk) << a.page_log2) + (there ? t & in_page : 0));
+    // The page of the lane's 8 tokens (8 g..) of a tile (behind the table's end its last).  Where a tile has one page it is the
+    // same for the whole wave and comes as a scalar, on a counter of its own
+    auto page_of = [&](int t0) {
+        const int t = t0 + (ONE_PAGE ? 0 : 8 * g);
+        const int at = t >> a.page_log2;
+        return table[at < last ? at : last];
+    };
+    auto there_at = [&](int page) { return (unsigned)page < (unsigned)a.n_pages; };
+    // the vector of token t, a multiple of 8, in the cache; of token 0 of page 0 where there is no such page
+    auto vector_at = [&](int t, int page) {
+        const bool there = there_at(page);
+        return (((long long)((there ? page : 0) * (long long)a.hk + hk)) << a.page_log2) + (there ? t & in_page : 0);
+    };
+    uint4 kr[2][KL];
+    unsigned vreg[8][VW];
+    float ks[8], vs[8];
+    const int key_row = 8 * (n >> 2) + (n & 3);
+    auto load_keys = [&](int t0, int page) {
+        auto from = [&](const unsigned char* p, int off) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int s = 0; s < KL; ++s) kr[u][s] = KL > 1 && SCALED ? *reinterpret_cast<const uint4*>(p + (off + 4 * u * row + key_at[s])) : streamed<uint4>(p + (off + 4 * u * row + key_at[s]));
+        };
+        if constexpr (ONE_PAGE) {
+            const long long at = vector_at(t0, page);
+            from(kc + at * row, key_row * row);
+            if constexpr (SCALED) bh_load8(a.k_scale + at + 8 * g, ks);
+        } else {
+            const int key_page = __shfl(page, 16 * (n >> 2));  // of the lanes whose own tokens these are
+            from(kc + vector_at(t0 + 8 * (n >> 2), key_page) * row, (n & 3) * row);
+            if constexpr (SCALED) bh_load8(a.k_scale + vector_at(t0 + 8 * g, page), ks);
+        }
+    };
+    auto load_values = [&](int t0, int page) {
+        auto from = [&](const unsigned char* p, int off) {
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                const unsigned char* q = p + (off + r * row);
+                if constexpr (VW == 1) {
+                    vreg[r][0] = streamed<unsigned>(q);
+                } else if constexpr (VW == 2) {
+                    const uint2 x = streamed<uint2>(q);
+                    vreg[r][0] = x.x, vreg[r][1] = x.y;
+                } else {
+#pragma unroll
+                    for (int w = 0; w < VW; w += 4) {
+                        const uint4 x = streamed<uint4>(q + 4 * w);
+                        vreg[r][w] = x.x, vreg[r][w + 1] = x.y, vreg[r][w + 2] = x.z, vreg[r][w + 3] = x.w;
+                    }
+                }
+            }
+        };
+        if constexpr (ONE_PAGE) {
+            const long long at = vector_at(t0, page);
+            from(vc + at * row, 8 * g * row + value_at);
+            if constexpr (SCALED) bh_load8(a.v_scale + at + 8 * g, vs);
+        } else {
+            const long long at = vector_at(t0 + 8 * g, page);
+            from(vc + at * row, value_at);
+            if constexpr (SCALED) bh_load8(a.v_scale + at, vs);
+        }
     };
 
     // lo can be zero or below: an infinite value, times it, spoils what hi made of it.  Where a sum came out as NaN, the walk is taken once
@@ -184,51 +261,33 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) bh_paged_attent
         m = -INFINITY, total = 0.f, v_top = 0x1p-126f;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) o[j] = floatx4{0.f, 0.f, 0.f, 0.f};
-        for (int t0 = lo + wave * TILE; t0 < hi; t0 += WAVES * TILE) {
-            bool there, key_there;
-            const long long kv = vector_at(t0 + 8 * (n >> 2), key_there) + (n & 3);  // keys of row n: + 4 in the second tile
-            const long long vv = vector_at(t0 + 8 * g, there);                       // the lane's 8 tokens
-            uint4 kr[2][KL];
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int s = 0; s < KL; ++s) {
-                    const int byte = 16 * (4 * s + g);
-                    kr[u][s] = uint4{0, 0, 0, 0};
-                    if (key_there && byte < row) kr[u][s] = *reinterpret_cast<const uint4*>(kc + (kv + 4 * u) * row + byte);
-                }
-            unsigned vreg[8][VW];
-#pragma unroll
-            for (int r = 0; r < 8; ++r) {
-#pragma unroll
-                for (int w = 0; w < VW; ++w) vreg[r][w] = 0;
-                const bool want = there && t0 + 8 * g + r < hi && t0 + 8 * g + r >= start && NJ * n < a.dim;
-                if (want) {
-                    const unsigned char* p = vc + (vv + r) * row + NJ * ES * n;
-                    if constexpr (VW == 1) {
-                        vreg[r][0] = *reinterpret_cast<const unsigned*>(p);
-                    } else if constexpr (VW == 2) {
-                        const uint2 x = *reinterpret_cast<const uint2*>(p);
-                        vreg[r][0] = x.x, vreg[r][1] = x.y;
-                    } else {
-#pragma unroll
-                        for (int w = 0; w < VW; w += 4) {
-                            const uint4 x = *reinterpret_cast<const uint4*>(p + 4 * w);
-                            vreg[r][w] = x.x, vreg[r][w + 1] = x.y, vreg[r][w + 2] = x.z, vreg[r][w + 3] = x.w;
-                        }
-                    }
-                }
-            }
-            float ks[8], vs[8];
-            if constexpr (SCALED) {
-#pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    ks[r] = there ? a.k_scale[vv + r] : 0.f;
-                    vs[r] = there && t0 + 8 * g + r < hi && t0 + 8 * g + r >= start ? a.v_scale[vv + r] : 0.f;
-                }
-            }
+        int t0 = lo + wave * TILE;
+        int next_page = 0;
+        bool there = false;
+        if (t0 < hi) {
+            const int page = page_of(t0);
+            next_page = page_of(t0 + WAVES * TILE);
+            there = there_at(page);
+            load_keys(t0, page);
+            load_values(t0, page);
+        }
+        // A tile's keys are asked for as soon as the tile before has used its own, its values likewise: no registers but one tile's.  Its
+        // pages are asked for a tile earlier, before those loads: loads come back in order, and a page asked for behind a tile's values
+        // would make the next tile's keys wait for them
+        while (t0 < hi) {
+            const int next = t0 + WAVES * TILE;
+            int after_page = 0;
+            const bool whole = t0 >= start && t0 + TILE <= hi && __all(there);
 
             // ---- S^T
+            if (!EXACT) {
+#pragma unroll
+                for (int s = 0; s < KL; ++s)
+                    if (16 * (4 * s + g) >= row) kr[0][s] = kr[1][s] = uint4{0, 0, 0, 0};
+            }
+            int q_lane = lane;
+            // (or the loads move out of the loop, into the registers that they are to spare; heads of 64 have those)
+            if constexpr (DP > 64) asm volatile("" : "+v"(q_lane));
             floatx4 st[2] = {floatx4{0.f, 0.f, 0.f, 0.f}, floatx4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
             for (int u = 0; u < 2; ++u)
@@ -243,65 +302,79 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) bh_paged_attent
                     } else {
                         kf = __builtin_bit_cast(frag, kr[u][s]);
                     }
-                    st[u] = Mma<M>::mul(kf, qf[s], st[u]);
+                    st[u] = Mma<M>::mul(kf, sh_q[s][q_lane], st[u]);
                 }
+            float x[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) x[r] = st[r >> 2][r & 3] * (SCALED ? ks[r] * unit : unit);
+            if (next < hi) {
+                after_page = page_of(next + WAVES * TILE);
+                load_keys(next, next_page);
+            }
 
             // ---- softmax: the lane's 8 tokens of head n
-            float x[8];
-            float top = -INFINITY;
+            if (a.softcap > 0.f) {
 #pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                const int t = t0 + 8 * g + r;
-                float dot = st[r >> 2][r & 3];
-                if constexpr (SCALED) dot *= ks[r];
-                float y = dot * unit;
-                if (a.softcap > 0.f) {
-                    const float e2 = __builtin_amdgcn_exp2f(fminf(y * cap_unit, 64.f));  // e^(2 s / c)
-                    y = y == y ? cap * (e2 - 1.f) * __builtin_amdgcn_rcpf(e2 + 1.f) : y;
+                for (int r = 0; r < 8; ++r) {
+                    const float e2 = __builtin_amdgcn_exp2f(fminf(x[r] * cap_unit, 64.f));  // e^(2 s / c)
+                    x[r] = x[r] == x[r] ? cap * (e2 - 1.f) * __builtin_amdgcn_rcpf(e2 + 1.f) : x[r];
                 }
-                y -= slope * (float)(len - 1 - t);
-                x[r] = there && t < hi && t >= start ? y : -INFINITY;
-                top = fmaxf(top, x[r]);
             }
-            const float now = fmaxf(m, over_groups_max(top));
-            const float base = now == -INFINITY ? 0.f : now;
-            float fade = __builtin_amdgcn_exp2f(m - base);
-            m = now;
-            float per = 1.f;
+            if (a.slopes) {
+                const float by = DP > 64 ? sh_stats[wave][0][n] : slope;
+#pragma unroll
+                for (int r = 0; r < 8; ++r) x[r] -= by * (float)(len - 1 - t0 - 8 * g - r);
+            }
+            if (!whole) {
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    const int t = t0 + 8 * g + r;
+                    const bool counts = there && t < hi && t >= start;
+                    if (!counts) {
+                        x[r] = -INFINITY;
+                        if (SCALED) vs[r] = 0.f;
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) vreg[r][w] = 0;
+                    }
+                }
+            }
+            float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+            if (__any(top > m)) {  // (a few times at the start of a walk, then hardly ever)
+                const float now = fmaxf(m, over_groups_max(top));
+                const float fade = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - now);
+                m = now;
+                total *= fade;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) o[j] *= fade;
+            }
             if constexpr (SCALED) {
-                float big = vs[0];
+                const float big = fmaxf(fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])), fmaxf(fmaxf(vs[4], vs[5]), fmaxf(vs[6], vs[7])));
+                if (__any(big > v_top)) {
+                    // the power of two at or above the largest scale of the wave's tokens so far
+                    const unsigned b = __float_as_uint(over_groups_max(big));
+                    const float up = __uint_as_float((b & 0x7f800000u) + ((b & 0x7fffffu) && b < 0x7f000000u ? 0x800000u : 0u));
+                    const float to = fmaxf(v_top, up), shrink = v_top / to;
 #pragma unroll
-                for (int r = 1; r < 8; ++r) big = fmaxf(big, vs[r]);
-                big = over_groups_max(big);
-                // the power of two at or above it
-                const unsigned b = __float_as_uint(big);
-                const float up = __uint_as_float((b & 0x7f800000u) + ((b & 0x7fffffu) && b < 0x7f000000u ? 0x800000u : 0u));
-                const float next = fmaxf(v_top, up);
-                const float shrink = v_top / next;
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) o[j] *= shrink;
-                v_top = next;
-                per = 1.f / next;
+                    for (int j = 0; j < NJ; ++j) o[j] *= shrink;
+                    v_top = to;
+                }
             }
-            float p[8];
-            total *= fade;
-#pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                p[r] = __builtin_amdgcn_exp2f(x[r] - base);
-                total += p[r];
-                p[r] *= (F16 ? 0x1p14f : 1.f);
-                if constexpr (SCALED) p[r] *= vs[r] * per;
-            }
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) o[j] *= fade;
+            const float base = m == -INFINITY ? 0.f : m - HOLD, per = 1.f / v_top;
             frag hi_p, lo_p;
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
+                float p = __builtin_amdgcn_exp2f(x[r] - base);
+                total += p;
+                if constexpr (SCALED) p *= vs[r] * per;
                 // one value for both: left alone, the compiler rounds the product above to fp16 once in a fused instruction for hi and once
                 // by way of fp32 for what hi is subtracted from, and where those fall on different sides lo belongs to another hi
-                asm("" : "+v"(p[r]));
-                hi_p[r] = (M)p[r];
-                lo_p[r] = both ? (M)(p[r] - (float)hi_p[r]) : (M)0.f;
+                asm("" : "+v"(p));
+                hi_p[r] = (M)p;
+                lo_p[r] = (M)(p - (float)hi_p[r]);
+            }
+            if (!both) {
+#pragma unroll
+                for (int r = 0; r < 8; ++r) lo_p[r] = (M)0.f;
             }
 
             // ---- O^T
@@ -335,24 +408,29 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) bh_paged_attent
                     f0.w = __builtin_amdgcn_perm(vreg[7][w], vreg[6][w], 0x05040100u), f1.w = __builtin_amdgcn_perm(vreg[7][w], vreg[6][w], 0x07060302u);
                     const frag v0 = __builtin_bit_cast(frag, f0), v1 = __builtin_bit_cast(frag, f1);
                     o[2 * w] = Mma<M>::mul(v0, hi_p, o[2 * w]);
-                    if (both) o[2 * w] = Mma<M>::mul(v0, lo_p, o[2 * w]);
                     o[2 * w + 1] = Mma<M>::mul(v1, hi_p, o[2 * w + 1]);
-                    if (both) o[2 * w + 1] = Mma<M>::mul(v1, lo_p, o[2 * w + 1]);
+                    if (both) {
+                        o[2 * w] = Mma<M>::mul(v0, lo_p, o[2 * w]);
+                        o[2 * w + 1] = Mma<M>::mul(v1, lo_p, o[2 * w + 1]);
+                    }
                 }
             }
+            if (next < hi) load_values(next, next_page);
+            t0 = next, there = there_at(next_page), next_page = after_page;
         }
         if (SCALED || !both) break;
         bool odd = false;
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) odd |= o[j][r] != o[j][r];
+            for (int r = 0; r < 4; ++r) odd |= o[j][r] != o[j][r] && (EXACT || NJ * (4 * g + r) + j < a.dim);
         if (!__any(odd)) break;
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) sh_out[wave][n][NJ * (4 * g + r) + j] = o[j][r];
     }
+    total *= F16 ? 0x1p-14f : 1.f;
 
     // ---- the workgroup's waves joined
     total = over_groups_sum(total);
@@ -365,7 +443,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) bh_paged_attent
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) all = fmaxf(all, sh_stats[w][0][n]);
     const float base = all == -INFINITY ? 0.f : all;
-    const float mine = __builtin_amdgcn_exp2f(m - base - HOLD) * (SCALED ? v_top : 1.f);
+    const float mine = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - base - HOLD) * (SCALED ? v_top : 1.f);
     // lane (g, n), tile j, element r: head n, dim NJ (4 g + r) + j
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
@@ -401,11 +479,13 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) bh_paged_attent
     }
 }
 
-// Joins the splits of one query head: a workgroup a head, thread d its dim (and the splits by turns, where there are threads left).
+// Joins the splits of one query head: a workgroup a head.  The splits' weights go to LDS; then 4 dims a thread, the splits by turns (8 of them
+// at a time for a head of 128), 4 loads in flight.
 template <typename E>
 __global__ void __launch_bounds__(256) bh_paged_attention_join_kernel(PagedArgs a) {
-    __shared__ float sh[256];
-    __shared__ float sh_sum;
+    extern __shared__ __attribute__((aligned(16))) float weight[];  // [splits]
+    __shared__ float sh[4];
+    __shared__ floatx4 sh_out[256];
     const int head = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x;
     int len = a.lengths[seq];
     const long long most = (long long)a.table_width << a.page_log2;
@@ -423,54 +503,72 @@ __global__ void __launch_bounds__(256) bh_paged_attention_join_kernel(PagedArgs 
     top = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
     const float from = top == -INFINITY ? 0.f : top;
     float sum = 0.f;
-    for (int s = tid; s < live; s += 256) sum += stats[2 * s + 1] * __builtin_amdgcn_exp2f(stats[2 * s] - from);
+    for (int s = tid; s < live; s += 256) {
+        const float w = __builtin_amdgcn_exp2f(stats[2 * s] - from);
+        weight[s] = w;
+        sum += stats[2 * s + 1] * w;
+    }
     sum = bh_group_sum(sum, 64);
     __syncthreads();
     if ((tid & 63) == 0) sh[tid >> 6] = sum;
     __syncthreads();
-    if (tid == 0) sh_sum = sh[0] + sh[1] + sh[2] + sh[3];
-    __syncthreads();
-    sum = sh_sum;
-    const int wide = 1 << (32 - __clz(a.dim - 1));  // threads of one split: a power of two, 16..256
+    sum = sh[0] + sh[1] + sh[2] + sh[3];
+    const int quads = a.dim >> 2, wide = 1 << (32 - __clz(quads - 1));  // threads of one split: a power of two, 4..64
     const int d = tid & (wide - 1), turns = 256 / wide;
-    float x = 0.f;
-    if (d < a.dim)
-        for (int s = tid / wide; s < live; s += turns)
-            x += a.part_out[(at * a.splits + s) * a.dim + d] * __builtin_amdgcn_exp2f(stats[2 * s] - from);
-    sh[tid] = x;
+    floatx4 x = {0.f, 0.f, 0.f, 0.f};
+    if (d < quads) {
+        const floatx4* part = reinterpret_cast<const floatx4*>(a.part_out + at * a.splits * a.dim) + d;
+#pragma unroll 4
+        for (int s = tid / wide; s < live; s += turns) x += part[(long long)s * quads] * weight[s];
+    }
+    sh_out[tid] = x;
     __syncthreads();
     if (tid < a.dim) {
-        for (int i = 1; i < turns; ++i) x += sh[tid + i * wide];
-        static_cast<E*>(a.out)[at * a.dim + tid] = (E)(sum > 0.f || sum != sum ? x / sum : 0.f);
+        float y = 0.f;
+        for (int i = 0; i < turns; ++i) y += sh_out[(tid >> 2) + i * wide][tid & 3];
+        static_cast<E*>(a.out)[at * a.dim + tid] = (E)(sum > 0.f || sum != sum ? y / sum : 0.f);
         if (tid == 0 && a.lse) a.lse[at] = sum > 0.f || sum != sum ? LN2 * (top + __builtin_amdgcn_logf(sum)) : -INFINITY;
     }
 }
 
-// How the cache's length is split: about 2048 workgroups (8 on each CU) at the longest that the table allows, in splits of 128 tokens
-// and more; a sequence uses as many of them as its own length fills.
+// How the cache's length is split, by the longest length that the table allows (the lengths themselves are on the device); a sequence uses
+// as many splits as its own length fills.  A CU takes about 30 GB/s whatever runs on it (700 tokens of one key head in one workgroup of 4
+// waves or of 8: 12 us), so few sequences are spread over all 256 of them, down to 128 tokens a workgroup (one tile a wave: 6.7 us); beyond
+// that fewer, longer splits cost less (64 sequences, up to 8191 tokens: 194 / 187 / 192 us in splits of 512 / 1024 / 2048; a window of
+// 4096 on 444 heads: 41 / 43 / 53).  The join is a second launch of 3.7 us and more: none up to 768 tokens (8 heads, 700 tokens: 12.0 against 6.6 + 3.7
+// and a launch), nor up to 2048 where the sequences alone fill the chip (32 sequences, up to 2000 tokens: 43.4 against 45.4 + 4.6).
 void split_length(int64_t batch, int64_t blocks, int64_t longest, int32_t window, int* splits, int* per_split) {
     if (window > 0 && window + TILE < longest) longest = window + TILE;  // (a window's start is rounded down to a tile)
-    const int64_t step = WAVES * TILE, work = batch * blocks;
-    int64_t want = (2048 + work - 1) / work;
-    int64_t per = (longest + want - 1) / want;
-    per = (per + step - 1) / step * step;
-    if (per < step) per = step;
-    if (per < 512 && longest > 512 && work * ((longest + 511) / 512) >= 512) per = 512;
-    *per_split = (int)per;
-    const int64_t n = (longest + per - 1) / per;
+    const int64_t work = batch * blocks, step = WAVES * TILE;
+    int64_t per = (longest * work / 256 + step - 1) / step * step;
+    per = per < step ? step : per > 1024 ? 1024 : per;
+    if (longest <= 768 || (longest <= 2048 && work >= 256)) per = (longest + step - 1) / step * step;
+    if (longest > per * 4096) per = (longest / 4096 + step) / step * step;  // (the join holds the splits' weights in LDS)
+    *per_split = (int)(per < step ? step : per);
+    const int64_t n = (longest + *per_split - 1) / *per_split;
     *splits = (int)(n < 1 ? 1 : n);
+}
+
+template <typename E, int CACHE, int DP, bool EXACT>
+void launch_split(const PagedArgs& a, hipStream_t st) {
+    const dim3 grid(a.hk * a.blocks, a.batch, a.splits), block(64 * WAVES);
+    if (a.page_log2 >= 5)
+        hipLaunchKernelGGL((bh_paged_attention_kernel<E, CACHE, DP, EXACT, true>), grid, block, 0, st, a);
+    else
+        hipLaunchKernelGGL((bh_paged_attention_kernel<E, CACHE, DP, EXACT, false>), grid, block, 0, st, a);
 }
 
 template <typename E, int CACHE>
 void launch_dim(const PagedArgs& a, hipStream_t st) {
-    const dim3 grid(a.splits, a.hk * a.blocks, a.batch), block(64 * WAVES);
-    if (a.dim <= 64)
-        hipLaunchKernelGGL((bh_paged_attention_kernel<E, CACHE, 64>), grid, block, 0, st, a);
-    else if (a.dim <= 128)
-        hipLaunchKernelGGL((bh_paged_attention_kernel<E, CACHE, 128>), grid, block, 0, st, a);
+    if (a.dim == 64)
+        launch_split<E, CACHE, 64, true>(a, st);
+    else if (a.dim == 128)
+        launch_split<E, CACHE, 128, true>(a, st);
+    else if (a.dim < 128)
+        launch_split<E, CACHE, 128, false>(a, st);
     else
-        hipLaunchKernelGGL((bh_paged_attention_kernel<E, CACHE, 256>), grid, block, 0, st, a);
-    if (a.splits > 1) hipLaunchKernelGGL((bh_paged_attention_join_kernel<E>), dim3(a.hq, a.batch), dim3(256), 0, st, a);
+        launch_split<E, CACHE, 256, false>(a, st);
+    if (a.splits > 1) hipLaunchKernelGGL((bh_paged_attention_join_kernel<E>), dim3(a.hq, a.batch), dim3(256), a.splits * sizeof(float), st, a);
 }
 
 int check_sizes(int32_t batch, int32_t hq, int32_t hk, int32_t dim, int32_t page_size, int32_t width) {
@@ -515,6 +613,7 @@ int bh_op_paged_attention(const void* q, int64_t q_seq, int64_t q_head, int32_t 
     if (batch == 0) return BH_OK;
     if (!q || !lengths || !out || (table_width && (!table || !k_cache || !v_cache))) return bh_fail(BH_EINVAL, "null buffer");
     if (scaled && table_width && (!k_scale || !v_scale)) return bh_fail(BH_EINVAL, "an 8-bit cache needs the scales of keys and values");
+    if (!bh_aligned16(k_scale) || !bh_aligned16(v_scale)) return bh_fail(BH_EUNSUPPORTED, "scales must be 16-byte aligned");
     if (!bh_aligned16(q) || !bh_aligned16(k_cache) || !bh_aligned16(v_cache) || (q_seq | q_head) % 8)
         return bh_fail(BH_EUNSUPPORTED, "queries and cache must be 16-byte aligned");
     PagedArgs a{};
@@ -530,7 +629,7 @@ int bh_op_paged_attention(const void* q, int64_t q_seq, int64_t q_head, int32_t 
     a.part_out = static_cast<float*>(workspace);
     a.part_stats = a.part_out + parts * head_dim;
     a.batch = batch, a.hq = n_q_heads, a.hk = n_k_heads, a.dim = head_dim, a.n_pages = (int)n_pages;
-    a.page_log2 = bh_ceil_log2(page_size), a.table_width = table_width;
+    a.page_log2 = bh_ceil_log2(page_size), a.table_width = n_pages ? table_width : 0;
     a.window = window, a.scale = scale, a.softcap = softcap;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (dtype == BH_F16) {

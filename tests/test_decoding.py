@@ -128,7 +128,7 @@ def test_refused_by_the_c_entry_points():
     for code, k in [(E, dict(dtype=F)), (E, dict(cache=H)), (E, dict(cache=F)), (E, dict(batch=-1)), (E, dict(hq=7)), (E, dict(hk=0)), (U, dict(dim=72)),
                     (U, dict(dim=272)), (U, dict(page=4)), (U, dict(page=48)), (E, dict(width=-1)), (U, dict(batch=65536)), (U, dict(width=1 << 30)),
                     (E, dict(s=math.nan)), (E, dict(cap=-1.0)), (E, dict(cap=math.inf)), (E, dict(cap=math.nan)), (E, dict(window=-1)), (E, dict(q=None)),
-                    (E, dict(kc=None)), (E, dict(cache=E4)), (E, dict(pages=-1)), (U, dict(q=ctypes.c_void_p(4098))), (U, dict(q_seq=511)),
+                    (E, dict(kc=None)), (E, dict(cache=E4)), (E, dict(pages=-1)), (U, dict(cache=I8, scale=ctypes.c_void_p(4100))), (U, dict(q=ctypes.c_void_p(4098))), (U, dict(q_seq=511)),
                     (E, dict(width=4096, n=1024)), (E, dict(width=4096, ws=None)), (E, dict(width=4096, ws=ctypes.c_void_p(4104)))]:
         assert attend(**k) == code, k
         assert lib.bh_last_error(), k
