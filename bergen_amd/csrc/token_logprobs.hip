@@ -5,8 +5,8 @@
 // A wave keeps ONE running maximum m for its 64 lanes (it changes a handful of times over a row; a maximum per lane would change in
 // some lane at nearly every step) and per lane the sums of e^(x - m) and (x - m) e^(x - m) in fp32.  The sum leaves out the
 // maximum's own 1: log1p of the rest keeps the entropy of a row that is nearly certain.
-// Top alternatives: the wave's 64 best (value, index) keys live sorted across its lanes; a block of 8 elements per lane is looked at
-// only if its maximum beats the k-th key, what does goes into a buffer in LDS, and 64 of those are sorted in at a time.
+// Top alternatives: the wave's 64 best (value, index) keys live sorted across its lanes; elements are looked at only where the step's
+// maximum beats the k-th key, and each that does takes its place at once, so that the bar is never stale (about k ln(n / 2048) of a wave's n).
 // -inf (banned tokens) carries no probability; a row of nothing else has log probabilities -inf and entropy 0.  A row that holds a
 // NaN or +inf has NaN log probabilities and entropy; its alternatives are ordered with NaN below -inf.  Ties go to the lower index.
 // Bound: HBM (every logit is read once); ~9 vector instructions per logit.
@@ -47,84 +47,86 @@ __device__ __forceinline__ Seen joined(const Seen& a, const Seen& b) {
     return r;
 }
 
-// Order of the alternatives: the key of value x at index i; NaN is below -inf.  0 is no key at all.
+// Order of the alternatives: the key of value x at index i; NaN is below -inf, and -0 is 0.  0 is no key at all.
 __device__ __forceinline__ u64 key_of(float x, int i) {
-    return ((u64)(x == x ? bh_ordf(x) : BH_ORD_NEG_INF - 1) << 32) | (u64)(~(unsigned)i);
+    return ((u64)(x == x ? bh_ordf(x + 0.0f) : BH_ORD_NEG_INF - 1) << 32) | (u64)(~(unsigned)i);
 }
 
 template <typename E>
 struct Vec {
     static constexpr int N = 16 / sizeof(E);
+    typedef E type __attribute__((ext_vector_type(N)));
 };
 
-// The elements of 16-byte vector v of a row whose first element sits `off` elements behind a 16-byte border; what lies outside the
-// row comes as -inf and has no index in [0, vocab).
+// The 16-byte vector v of a row whose first element sits `off` elements behind a 16-byte border; what lies outside the row, or behind
+// the part's last vector, comes as -inf.
 template <typename E>
-__device__ __forceinline__ void load_vector(const E* row, int off, int vocab, long long v, float (&x)[Vec<E>::N]) {
+__device__ __forceinline__ typename Vec<E>::type load_vector(const E* row, int off, int vocab, long long v, long long v1) {
+    typedef typename Vec<E>::type vec;
     constexpr int N = Vec<E>::N;
     const long long e0 = v * N - off;
-    if (e0 >= 0 && e0 + N <= vocab) {
-        typedef E vec __attribute__((ext_vector_type(N)));
-        const vec w = *reinterpret_cast<const vec*>(row + e0);
-#pragma unroll
-        for (int e = 0; e < N; ++e) x[e] = (float)w[e];
+    vec w;
+    if (v < v1 && e0 >= 0 && e0 + N <= vocab) {
+        w = __builtin_nontemporal_load(reinterpret_cast<const vec*>(row + e0));
     } else {
 #pragma unroll
-        for (int e = 0; e < N; ++e) x[e] = e0 + e >= 0 && e0 + e < vocab ? (float)row[e0 + e] : -INFINITY;
+        for (int e = 0; e < N; ++e) w[e] = v < v1 && e0 + e >= 0 && e0 + e < vocab ? row[e0 + e] : (E)-INFINITY;
     }
+    return w;
 }
 
-// What the waves of a workgroup found, joined by its first wave and written down: as the row's result, or as one part of it.
+// What a workgroup joins: the distributions its waves (or a row's parts) saw and, in `sorted` lists of `top` keys, their best.
+template <int KEYS>
 struct Shared {
-    float stats[WAVES][4];
-    u64 keys[WAVES][64];
+    alignas(16) float stats[WAVES][4];
+    u64 bar, low;
+    int count;
+    u64 keys[KEYS];
 };
 
-__device__ __forceinline__ void finish(const LogprobArgs& a, int row, int part, int parts, Shared& sh, int lane, int wave, const Seen& mine, u64 key) {
-    if (lane == 0) {
-        sh.stats[wave][0] = mine.m;
-        sh.stats[wave][1] = mine.rest;
-        sh.stats[wave][2] = mine.first;
-        sh.stats[wave][3] = mine.bad ? 1.f : 0.f;
-    }
-    if (a.top) sh.keys[wave][lane] = key;
+// The best `top` of n_lists sorted lists, out(rank, key) for each, by the whole workgroup: what reaches a bar that `top` keys reach is
+// collected and ranked by counting.  Two bars do: the best of the lists' last keys (`top` keys of that list), which is the higher one for few lists, and
+// the least of their r-th, r = top / n_lists rounded up (r keys of each), for many.  Ranks that have no key: out(rank, 0).
+template <int KEYS, typename Get, typename Out>
+__device__ __forceinline__ void join_lists(Shared<KEYS>& sh, int n_lists, int top, Get get, Out out) {
+    const int tid = threadIdx.x;
+    if (tid == 0) sh.bar = 0, sh.low = ~0ull, sh.count = 0;
     __syncthreads();
-    if (wave) return;
-    Seen s = mine;
-    for (int w = 1; w < WAVES; ++w) s = joined(s, Seen{sh.stats[w][0], sh.stats[w][1], sh.stats[w][2], sh.stats[w][3] != 0.f});
-    if (a.top) {
-        u64 acc[1] = {key};
-        for (int w = 1; w < WAVES; ++w) {
-            const u64 b[1] = {sh.keys[w][lane]};
-            bh_wave_merge_top<1>(acc, b, lane);
-        }
-        key = acc[0];
+    const int r = (top + n_lists - 1) / n_lists;
+    for (int l = tid; l < n_lists; l += THREADS) {
+        atomicMax(&sh.bar, get(l, top - 1));
+        atomicMin(&sh.low, get(l, r - 1));
     }
-    if (parts > 1) {
-        const long long at = (long long)row * parts + part;
-        if (lane == 0) *reinterpret_cast<floatx4*>(a.part_stats + 4 * at) = floatx4{s.m, s.rest, s.first, s.bad ? 1.f : 0.f};
-        if (lane < a.top) a.part_keys[at * a.top + lane] = key;
-        return;
+    __syncthreads();
+    const u64 bar = sh.bar > sh.low ? sh.bar : sh.low;
+    for (int i = tid; i < n_lists * top; i += THREADS) {
+        const int l = i / top;
+        const u64 k = get(l, i - l * top);
+        if (k && k >= bar) sh.keys[atomicAdd(&sh.count, 1)] = k;
     }
+    __syncthreads();
+    const int n = sh.count;
+    for (int i = tid; i < n; i += THREADS) {
+        const u64 k = sh.keys[i];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) rank += sh.keys[j] > k ? 1 : 0;
+        if (rank < top) out(rank, k);
+    }
+    for (int i = n + tid; i < top; i += THREADS) out(i, 0);
+}
+
+// A row's results, by the whole workgroup: `lists` sorted lists of keys, and what was seen in sh.stats.
+template <typename E, int KEYS, typename Get>
+__device__ __forceinline__ void finish(const LogprobArgs& a, int row, Shared<KEYS>& sh, int lists, Get get) {
+    Seen s{-INFINITY, 0.f, 0.f, false};
+    for (int w = 0; w < WAVES; ++w) s = joined(s, Seen{sh.stats[w][0], sh.stats[w][1], sh.stats[w][2], sh.stats[w][3] != 0.f});
     const float log_sum = log1pf(s.rest);
     const bool bad = s.bad || s.m == INFINITY, none = s.m == -INFINITY;
     const float gone = bad ? __uint_as_float(0x7fc00000u) : -INFINITY;  // of every token of a bad or an empty row
-    if (lane == 0) a.entropy[row] = bad ? gone : none ? 0.f : log_sum - LN2 * s.first / (1.0f + s.rest);
-    if (lane < a.top) {
-        const unsigned o = (unsigned)(key >> 32);
-        const float x = bh_unordf(o);
-        a.top_ids[(long long)row * a.top + lane] = (long long)bh_key_row(key);
-        a.top_logprobs[(long long)row * a.top + lane] = bad || none ? gone : (x - s.m) - log_sum;
-    }
-}
-
-// log probabilities of the row's given tokens; every lane of the wave that finish() leaves has the result's parts again from LDS
-template <typename E>
-__device__ __forceinline__ void given_tokens(const LogprobArgs& a, int row, const Seen& s, int lane) {
+    if (threadIdx.x == 0) a.entropy[row] = bad ? gone : none ? 0.f : log_sum - LN2 * s.first / (1.0f + s.rest);
     const E* x = static_cast<const E*>(a.x) + row * a.stride;
-    const float log_sum = log1pf(s.rest);
-    const bool bad = s.bad || s.m == INFINITY, none = s.m == -INFINITY;
-    for (int g = lane; g < a.given; g += 64) {
+    for (int g = threadIdx.x; g < a.given; g += THREADS) {
         const long long t = a.targets[(long long)row * a.given + g];
         float r = 0.f;  // a negative target names no token
         if (t >= a.vocab || (t >= 0 && bad))
@@ -133,6 +135,11 @@ __device__ __forceinline__ void given_tokens(const LogprobArgs& a, int row, cons
             r = none ? -INFINITY : ((float)x[t] - s.m) - log_sum;
         a.logprobs[(long long)row * a.given + g] = r;
     }
+    if (a.top)
+        join_lists(sh, lists, a.top, get, [&](int rank, u64 key) {
+            a.top_ids[(long long)row * a.top + rank] = (long long)bh_key_row(key);
+            a.top_logprobs[(long long)row * a.top + rank] = bad || none ? gone : (bh_key_score(key) - s.m) - log_sum;
+        });
 }
 
 __device__ __forceinline__ float wave_max(float v) {
@@ -140,11 +147,37 @@ __device__ __forceinline__ float wave_max(float v) {
     return v;
 }
 
+// the largest of three, NaN left out; as the one instruction (fmaxf first makes every operand that came from memory a quiet NaN if it is one)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+// the value of the lane before (lane 0: nothing that is used)
+__device__ __forceinline__ u64 lane_before(u64 v) {
+    const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)v, 0x138 /* wave_shr:1 */, 0xf, 0xf, false);
+    const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), 0x138, 0xf, 0xf, false);
+    return ((u64)hi << 32) | lo;
+}
+
+// A number that at least k of the wave's lanes reach with theirs, the largest with 16 leading bits only: found bit by bit by
+// counting (a full sort of the lanes takes four times as long, and a bar that is a little low lets one or two elements more through).
+__device__ __forceinline__ unsigned reached_by(unsigned v, int k) {
+    unsigned t = 0;
+    for (int bit = 31; bit >= 16; --bit) {
+        const unsigned c = t | (1u << bit);
+        if (__popcll(__ballot(v >= c)) >= k) t = c;
+    }
+    return t;
+}
+
 template <typename E, bool TOP>
-__global__ void __launch_bounds__(THREADS) bh_token_logprobs_kernel(LogprobArgs a) {
-    constexpr int N = Vec<E>::N, U = 4, HOLD = 64 + 64 * N;  // a buffer takes one block on top of what does not fill a list yet
-    __shared__ Shared sh;
-    __shared__ u64 buffer[TOP ? WAVES : 1][TOP ? HOLD : 1];
+__global__ void __launch_bounds__(THREADS, 4) bh_token_logprobs_kernel(LogprobArgs a) {
+    constexpr int MANY = 8, N = Vec<E>::N, U = 4;  // elements of a vector, vectors of a lane's step
+    typedef float Step __attribute__((ext_vector_type(U * N)));
+    __shared__ Shared<TOP ? WAVES * 64 : 1> sh;
+    __shared__ u64 lists[TOP ? WAVES * 64 : 1];  // the waves' own
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
     const E* x = static_cast<const E*>(a.x) + row * a.stride;
@@ -153,156 +186,192 @@ __global__ void __launch_bounds__(THREADS) bh_token_logprobs_kernel(LogprobArgs 
     const long long v0 = (long long)part * a.per_part;
     const long long v1 = v0 + a.per_part < vectors ? v0 + a.per_part : vectors;
 
-    Seen s{-INFINITY, 0.f, 0.f, false};  // m, bad: the wave's; rest, first: the lane's
+    Seen s{-INFINITY, 0.f, 0.f, false};  // m: the wave's; rest, first: the lane's
     float m2 = 0.f;                      // m log2(e), rounded (0 while there is nothing but -inf): what the exponents are taken from, and
     float off2 = 0.f;                    // what the rounding left of it: 2^off2 is the maximum's own weight, put right at the end
     u64 best = 0, bar = 0;               // the lane's key of the wave's list; the k-th key: what is not above it cannot be among the k
-    float bar_x = __uint_as_float(0x7fc00000u);  // its value; a NaN lets every block through
-    int held = 0;
-    bool first_block = true;
+    float bar_x = __uint_as_float(0x7fc00000u);  // its value; a NaN lets everything through
 
-    auto flush = [&]() {
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // other lanes of the wave wrote what this one reads
-        for (int at = 0; at < held; at += 64) {
-            u64 b[1] = {at + lane < held ? buffer[TOP ? wave : 0][at + lane] : 0}, acc[1] = {best};
-            bh_wave_sort_desc<1>(b, lane);
-            bh_wave_merge_top<1>(acc, b, lane);
-            best = acc[0];
+    // the indices of this part's elements; what lies outside (a row's ends, vectors that were not loaded) has none of them
+    const int i_first = v0 * N - off > 0 ? (int)(v0 * N - off) : 0;
+    const unsigned i_count = (unsigned)((v1 * N - off < a.vocab ? (int)(v1 * N - off) : a.vocab) - i_first);
+    // The elements of a step take their places in the list: those in its places `places` (bit b = u N + e: the lanes' elements e of their vectors
+    // u, index i0 + u THREADS N + e) that beat the bar.  Few places, as in all steps but the first: one after the other, the registers chosen
+    // by a scalar.  Many: one element of each lane at a time, read again, sorted and merged.  (Neither is there once for each of the 32 places: as it
+    // was, most of 37 us for 61 rows went into fetching instructions.  Which elements beat the bar is kept in scalars: as bits of
+    // each lane it took 24 vector instructions for a vector, not 8, and these are what the kernel is bound by.)
+    auto take = [&](const Step& xs, unsigned places, int i0) {
+        auto new_bar = [&]() {
+            const int k = a.top - 1;
+            const unsigned high = __builtin_amdgcn_readlane((int)(best >> 32), k);
+            const u64 kth = ((u64)high << 32) | (unsigned)__builtin_amdgcn_readlane((int)best, k);
+            if (kth > bar) bar = kth, bar_x = bh_unordf(high);
+        };
+        auto insert = [&](u64 key, unsigned long long who) {  // the keys of the lanes `who`, as long as they beat the bar
+            while (who) {
+                const int l = __ffsll(who) - 1;
+                const u64 k = ((u64)(unsigned)__builtin_amdgcn_readlane((int)(key >> 32), l) << 32) | (unsigned)__builtin_amdgcn_readlane((int)key, l);
+                const int at = __popcll(__ballot(best > k));
+                const u64 before = lane_before(best);
+                best = lane < at ? best : lane == at ? k : before;
+                new_bar();
+                who &= who - 1;
+                who &= __ballot(key > bar);
+            }
+        };
+        if (__popc(places) > MANY) {
+            unsigned look = 0;
+            for (; places; places &= places - 1) {
+                const int b = __ffs((int)places) - 1;
+                look |= !(xs[b] <= bar_x) ? 1u << b : 0;
+            }
+            for (; __any(look != 0); look &= look - 1) {
+                const int b = __ffs((int)look) - 1, i = i0 + (b / N) * THREADS * N + b % N;
+                u64 key[1] = {0}, acc[1] = {best};
+                if (look != 0 && (unsigned)(i - i_first) < i_count) key[0] = key_of((float)x[i], i);
+                const unsigned long long who = __ballot(key[0] > bar);
+                if (__popcll(who) > 12) {
+                    bh_wave_sort_desc<1>(key, lane);
+                    bh_wave_merge_top<1>(acc, key, lane);
+                    best = acc[0];
+                    new_bar();
+                } else {
+                    insert(key[0], who);
+                }
+            }
+            return;
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        held = 0;
-        const u64 kth = bh_shfl64(best, a.top - 1);
-        if (kth > bar) bar = kth;
-        if (bar) bar_x = bh_unordf((unsigned)(bar >> 32));
+        for (; places; places &= places - 1) {
+            const int b = __ffs((int)places) - 1, i = i0 + (b / N) * THREADS * N + b % N;
+            const u64 key = (unsigned)(i - i_first) < i_count ? key_of(xs[b], i) : 0;
+            insert(key, __ballot(key > bar));
+        }
     };
 
+    typename Vec<E>::type w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = load_vector(x, off, a.vocab, v0 + u * THREADS + threadIdx.x, v1);
     for (long long base = v0; base < v1; base += U * THREADS) {
-        float xs[U][N];
+        Step xs;
+        float most[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const long long v = base + u * THREADS + threadIdx.x;
-            if (v < v1)
-                load_vector(x, off, a.vocab, v, xs[u]);
-            else
 #pragma unroll
-                for (int e = 0; e < N; ++e) xs[u][e] = -INFINITY;
+            for (int e = 0; e < N; ++e) xs[u * N + e] = (float)w[u][e];
+            most[u] = N == 8 ? max3(max3(xs[u * N + 0], xs[u * N + 1], xs[u * N + 2]), max3(xs[u * N + 3], xs[u * N + 4], xs[u * N + 5]), max3(xs[u * N + 6], xs[u * N + 6], xs[u * N + N - 1]))
+                             : max3(xs[u * N + 0], xs[u * N + 1], max3(xs[u * N + 2], xs[u * N + 2], xs[u * N + 3]));
+        }
+        if (base + U * THREADS < v1) {  // the next step's loads run beside this one's arithmetic
+#pragma unroll
+            for (int u = 0; u < U; ++u) w[u] = load_vector(x, off, a.vocab, base + (U + u) * THREADS + threadIdx.x, v1);
+        }
+        const float step_most = max3(most[0], most[1], max3(most[2], most[2], most[3]));
+        if (TOP && __any(!(step_most <= bar_x))) {
+            if (base == v0) {
+                // a first bar, just below what k of the lanes' largest reach (k elements of the step are at least as good)
+                const unsigned o = step_most == step_most ? bh_ordf(step_most + 0.0f) : 0;
+                const unsigned kth = reached_by(o, a.top);
+                if (kth > BH_ORD_NEG_INF) {
+                    bar = ((u64)kth << 32) - 1;
+                    bar_x = bh_unordf(kth - (kth == 0x80000000u ? 2 : 1));  // (one below 0 is -0, which is not less)
+                }
+            }
+            unsigned places = 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (__any(!(most[u] <= bar_x))) {  // (what was seen before this step has lower indices: equal values stay out)
+#pragma unroll
+                    for (int e = 0; e < N; ++e) places |= __any(!(xs[u * N + e] <= bar_x)) ? 1u << (u * N + e) : 0;
+                }
+            take(xs, places, (int)((base + threadIdx.x) * N - off));
+        }
+        if (__any(step_most > s.m)) {  // a new maximum: a few times in a row
+            const float top_x = wave_max(step_most);
+            if (s.m > -INFINITY && top_x < INFINITY) {
+                const float by = m2 - __fmul_rn(top_x, LOG2E), f = __builtin_amdgcn_exp2f(by);
+                if (lane == 0) {  // the old maximum is one of many now
+                    const float own = __builtin_amdgcn_exp2f(off2);
+                    s.rest += own;
+                    s.first = fmaf(off2, own, s.first);
+                }
+                s.first = f > 0.f ? f * (s.first + by * s.rest) : 0.f;
+                s.rest *= f;
+            }
+            s.m = top_x;
+            m2 = __fmul_rn(top_x, LOG2E);
+            off2 = top_x < INFINITY ? fmaf(top_x, LOG2E, -m2) : 0.f;
+            // its own 1 is left out: one element that equals it, of one lane
+            bool mine = lane == __ffsll((unsigned long long)__ballot(step_most == top_x)) - 1;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (mine && xs[u * N + e] == top_x) {
+                        xs[u * N + e] = -INFINITY;
+                        mine = false;
+                    }
+            if (top_x == INFINITY) s.rest = __uint_as_float(0x7fc00000u);
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float most = xs[u][0];
-            bool nan = most != most;
-#pragma unroll
-            for (int e = 1; e < N; ++e) {
-                most = fmaxf(most, xs[u][e]);
-                nan |= xs[u][e] != xs[u][e];
-            }
-            const bool look = nan || !(most <= (TOP ? bar_x : s.m));
-            bool skip = false;  // the lane whose element became the maximum leaves its 1 out
-            if (__any(look)) {
-                if (__any(nan)) s.bad = true;
-                const float top_x = wave_max(most);
-                if (top_x > s.m) {
-                    if (s.m > -INFINITY && top_x < INFINITY) {
-                        const float by = m2 - __fmul_rn(top_x, LOG2E), f = __builtin_amdgcn_exp2f(by);
-                        if (lane == 0) {  // the old maximum is one of many now
-                            const float own = __builtin_amdgcn_exp2f(off2);
-                            s.rest += own;
-                            s.first = fmaf(off2, own, s.first);
-                        }
-                        s.first = f > 0.f ? f * (s.first + by * s.rest) : 0.f;
-                        s.rest *= f;
-                    }
-                    s.m = top_x;
-                    m2 = __fmul_rn(top_x, LOG2E);
-                    off2 = top_x < INFINITY ? fmaf(top_x, LOG2E, -m2) : 0.f;
-                    skip = lane == __ffsll((unsigned long long)__ballot(most == top_x)) - 1;
-                }
-                if (TOP) {
-                    const long long i0 = (base + u * THREADS + threadIdx.x) * N - off;
-                    const bool inside = base + u * THREADS + threadIdx.x < v1;
-                    if (first_block) {
-                        // a first bar: the k-th of the lanes' best elements (k of the block are at least as good)
-                        u64 k[1] = {0};
-#pragma unroll
-                        for (int e = 0; e < N; ++e)
-                            if (inside && i0 + e >= 0 && i0 + e < a.vocab) {
-                                const u64 ke = key_of(xs[u][e], (int)(i0 + e));
-                                k[0] = k[0] > ke ? k[0] : ke;
-                            }
-                        bh_wave_sort_desc<1>(k, lane);
-                        const u64 kth = bh_shfl64(k[0], a.top - 1);
-                        if (kth) {
-                            bar = kth - 1;
-                            bar_x = bh_unordf((unsigned)(bar >> 32));
-                        }
-                        first_block = false;
-                    }
-#pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        const u64 k = inside && i0 + e >= 0 && i0 + e < a.vocab ? key_of(xs[u][e], (int)(i0 + e)) : 0;
-                        const unsigned long long who = __ballot(k > bar);
-                        if (k > bar) buffer[wave][held + __popcll(who & ((1ull << lane) - 1))] = k;
-                        held += __popcll(who);
-                    }
-                    if (held >= 64) flush();
-                }
-            }
+        for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                const float t = fmaxf(fmaf(xs[u][e], LOG2E, -m2), -1000.0f);  // (-inf: 2^-1000 is 0, and so is its product)
-                float p = __builtin_amdgcn_exp2f(t);
-                if (skip && xs[u][e] == s.m) {
-                    p = 0.f;
-                    skip = false;
-                }
-                s.rest += p;
-                s.first = fmaf(t, p, s.first);
+                const float t = fmaf(xs[u * N + e], LOG2E, -m2), p = __builtin_amdgcn_exp2f(t);
+                s.rest += p;                              // (a NaN stays in it)
+                s.first = fmaf(fmaxf(t, -1000.0f), p, s.first);  // (-inf: p is 0, and so is its product with -1000)
             }
-        }
     }
-    if (TOP) flush();
     s.rest = bh_group_sum(s.rest, 64);
     s.first = bh_group_sum(s.first, 64);
+    s.bad = s.rest != s.rest;
     s.first = __builtin_amdgcn_exp2f(-off2) * (s.first - off2 * s.rest);  // from m2 to m itself
     s.rest *= __builtin_amdgcn_exp2f(-off2);
-    finish(a, row, part, a.parts, sh, lane, wave, s, best);
-    if (wave || a.parts > 1) return;
-    Seen all = s;
-    for (int w = 1; w < WAVES; ++w) all = joined(all, Seen{sh.stats[w][0], sh.stats[w][1], sh.stats[w][2], sh.stats[w][3] != 0.f});
-    given_tokens<E>(a, row, all, lane);
+    if (lane == 0) *reinterpret_cast<floatx4*>(sh.stats[wave]) = floatx4{s.m, s.rest, s.first, s.bad ? 1.f : 0.f};
+    if (TOP) lists[wave * 64 + lane] = best;
+    __syncthreads();
+    const auto get = [&](int l, int i) { return lists[TOP ? l * 64 + i : 0]; };
+    if (a.parts == 1) {
+        finish<E>(a, row, sh, WAVES, get);
+        return;
+    }
+    const long long at = (long long)row * a.parts + part;
+    if (threadIdx.x == 0) {
+        Seen all = s;
+        for (int w = 1; w < WAVES; ++w) all = joined(all, Seen{sh.stats[w][0], sh.stats[w][1], sh.stats[w][2], sh.stats[w][3] != 0.f});
+        *reinterpret_cast<floatx4*>(a.part_stats + 4 * at) = floatx4{all.m, all.rest, all.first, all.bad ? 1.f : 0.f};
+    }
+    if (TOP) join_lists(sh, WAVES, a.top, get, [&](int rank, u64 key) { a.part_keys[at * a.top + rank] = key; });
 }
 
-// Joins the parts of a row: one workgroup a row, wave w the parts w, w + 4, ...
+constexpr int JOIN_KEYS = 2048;  // parts times top: 16 KiB of LDS
+
+// Joins the parts of a row: one workgroup a row, wave w the distributions of its quarter of them.
 template <typename E>
 __global__ void __launch_bounds__(THREADS) bh_token_logprobs_join_kernel(LogprobArgs a) {
-    __shared__ Shared sh;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = blockIdx.x;
+    __shared__ Shared<JOIN_KEYS> sh;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.x;
     Seen s{-INFINITY, 0.f, 0.f, false};
-    u64 acc[1] = {0};
-    for (int p = wave; p < a.parts; p += WAVES) {
-        const long long at = (long long)row * a.parts + p;
-        const floatx4 f = *reinterpret_cast<const floatx4*>(a.part_stats + 4 * at);
+    for (int p = threadIdx.x; p < a.parts; p += THREADS) {
+        const floatx4 f = *reinterpret_cast<const floatx4*>(a.part_stats + 4 * ((long long)row * a.parts + p));
         s = joined(s, Seen{f[0], f[1], f[2], f[3] != 0.f});
-        if (a.top) {
-            const u64 b[1] = {lane < a.top ? a.part_keys[at * a.top + lane] : 0};
-            bh_wave_merge_top<1>(acc, b, lane);
-        }
     }
-    finish(a, row, 0, 1, sh, lane, wave, s, acc[0]);
-    if (wave) return;
-    Seen all = s;
-    for (int w = 1; w < WAVES; ++w) all = joined(all, Seen{sh.stats[w][0], sh.stats[w][1], sh.stats[w][2], sh.stats[w][3] != 0.f});
-    given_tokens<E>(a, row, all, lane);
+    for (int d = 1; d < 64; d <<= 1)
+        s = joined(s, Seen{__shfl_xor(s.m, d), __shfl_xor(s.rest, d), __shfl_xor(s.first, d), (bool)__shfl_xor((int)s.bad, d)});
+    if (lane == 0) *reinterpret_cast<floatx4*>(sh.stats[wave]) = floatx4{s.m, s.rest, s.first, s.bad ? 1.f : 0.f};
+    __syncthreads();
+    const u64* keys = a.part_keys + (long long)row * a.parts * a.top;
+    finish<E>(a, row, sh, a.parts, [&](int l, int i) { return keys[l * a.top + i]; });
 }
 
 // How a row is cut: enough workgroups for the chip (4 on each of 256 CUs) where there are few rows, parts of at least 4 vectors a
 // thread, whole steps of a workgroup.
-void cut(int64_t rows, int64_t vocab, int32_t dtype, int* parts, int* per_part) {
+void cut(int64_t rows, int64_t vocab, int32_t dtype, int32_t top, int* parts, int* per_part) {
     const int64_t n = 16 / (int64_t)bh_dtype_size(dtype);
     const int64_t vectors = (vocab + n - 1) / n + 1;  // (+ 1: a row that starts behind a 16-byte border)
     const int64_t step = 4 * THREADS, steps = (vectors + step - 1) / step;
     int64_t want = rows >= 1024 ? 1 : (1024 + rows - 1) / rows;
     if (want > steps) want = steps;
+    if (top > 0 && want > JOIN_KEYS / top) want = JOIN_KEYS / top;
     const int64_t per = (steps + want - 1) / want;
     *per_part = (int)(per * step);
     *parts = (int)((steps + per - 1) / per);
@@ -336,7 +405,7 @@ int64_t bh_op_token_logprobs_workspace(int64_t n_rows, int64_t vocab, int32_t dt
     if (rc) return rc;
     if (n_rows == 0) return 0;
     int parts, per;
-    cut(n_rows, vocab, dtype, &parts, &per);
+    cut(n_rows, vocab, dtype, top, &parts, &per);
     return parts > 1 ? n_rows * parts * (16 + 8 * (int64_t)top) : 0;
 }
 
@@ -352,7 +421,7 @@ int bh_op_token_logprobs(const void* logits, int64_t row_stride, int32_t dtype, 
         return bh_fail(BH_EINVAL, "null buffer");
     if ((uintptr_t)logits % bh_dtype_size(dtype)) return bh_fail(BH_EINVAL, "logits are not aligned to their type");
     LogprobArgs a{};
-    cut(n_rows, vocab, dtype, &a.parts, &a.per_part);
+    cut(n_rows, vocab, dtype, top, &a.parts, &a.per_part);
     const int64_t need = a.parts > 1 ? n_rows * a.parts * (16 + 8 * (int64_t)top) : 0;
     if (need && (!workspace || workspace_bytes < need || !bh_aligned16(workspace)))
         return bh_fail(BH_EINVAL, "workspace of %lld bytes, 16-byte aligned, needed: %lld given", (long long)need, (long long)workspace_bytes);

@@ -424,13 +424,16 @@ def test_logprobs_rows_and_ties(dtype):
     nan[5000], inf[123], both[1], both[2] = math.nan, math.inf, math.nan, math.inf
     few = torch.full((n,), math.nan)
     few[[10, 8000]] = torch.tensor([1.0, 2.0])
+    signs = torch.zeros(n)
+    signs[::3] = -0.0                                          # -0 and 0 are equal logits
+    rows.append(signs)
     x = torch.stack(rows + [one, banned, single, offset, nan, inf, both, few]).to(dtype).cuda()
     t = torch.tensor([0, 8999, 77, 4321, 10], device="cuda").expand(x.shape[0], 5).contiguous()
     for top in (1, 3, 50, 64):
         check_logprobs(x, t, top)
     r = bergen_amd.token_logprobs(x, t, top=3)
     assert r.top_ids[0].tolist() == [0, 1, 2] and r.entropy[3] == 0 and (r.logprobs[3] == -math.inf).all()
-    assert abs(float(r.entropy[0]) - math.log(n)) < 1e-5 and torch.isnan(r.logprobs[11]).all()
+    assert abs(float(r.entropy[0]) - math.log(n)) < 1e-5 and torch.isnan(r.logprobs[12]).all()
 
 
 def test_entropy_of_a_nearly_certain_row():
