@@ -1,10 +1,10 @@
 // decode_ops.hip — the memory-bound operators of a decoding step: RMS norm of query / key heads with rotary positions in the same
 // pass, and the paged key-value cache's write and read, plain or in 8 bits with a scale per token and head.
 //
-// All three move vectors of one (token, head): D elements, D <= 256.  The wide kernels give a lane 16 elements (two 16-byte
-// loads of 16-bit data) and a vector 2^ceil(log2(D / 16)) lanes, so that sums and maxima over a vector are 0..4 exchanges between
-// neighbouring lanes and nothing passes through LDS; they need D % 16 == 0 and 16-byte rows.  Everything else (odd
-// D, unaligned views) runs on the narrow kernels: one wave per vector, one element per lane and step.
+// All three move vectors of one (token, head): D elements, D <= 256.  The wide kernels give a lane two 16-byte pieces of a vector
+// and a vector 1..32 lanes, a power of two, so that sums and maxima over it are 0..5 exchanges between neighbouring lanes and nothing
+// passes through LDS; they need whole pieces and 16-byte rows.  Everything else (odd D, unaligned views) runs on the narrow
+// kernels: one wave per vector, one element per lane and step.
 // Bound: HBM (each element is read once and written once).
 #include "bh_decode.h"
 
@@ -40,19 +40,39 @@ __device__ __forceinline__ double position(const RotaryArgs& a, long long t) {
     return a.pos64 ? (double)static_cast<const long long*>(a.pos)[t] : (double)static_cast<const int*>(a.pos)[t];
 }
 
-template <typename E>
-__device__ __forceinline__ void weights8(const RotaryArgs& a, const void* w, int d, float (&x)[8]) {
-    if (a.w32)
-        bh_load8(static_cast<const float*>(w) + d, x);
-    else
-        bh_load8(static_cast<const E*>(w) + d, x);
+// C elements of E at p (of 16 bytes, or 8 where the other side is fp32) as fp32, and back, rounded once.
+template <typename E, int C>
+__device__ __forceinline__ void load16(const E* p, float (&x)[C]) {
+    typedef E vec __attribute__((ext_vector_type(C)));
+    const vec v = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+    for (int e = 0; e < C; ++e) x[e] = (float)v[e];
+}
+template <typename E, int C>
+__device__ __forceinline__ void store16(E* p, const float (&x)[C]) {
+    typedef E vec __attribute__((ext_vector_type(C)));
+    vec v;
+#pragma unroll
+    for (int e = 0; e < C; ++e) v[e] = (E)x[e];
+    *reinterpret_cast<vec*>(p) = v;
+}
+template <typename E, int C>
+__device__ __forceinline__ void weights(const RotaryArgs& a, const void* w, int d, float (&x)[C]) {
+    if (a.w32) {
+#pragma unroll
+        for (int e = 0; e < C; e += 4) load16<float, 4>(static_cast<const float*>(w) + d + e, reinterpret_cast<float(&)[4]>(x[e]));
+    } else {
+        load16<E, C>(static_cast<const E*>(w) + d, x);
+    }
 }
 
 // A workgroup takes `tb` tokens with all their heads: the sines of a token are computed once, into LDS, and shared by its heads
-// (64 for a head of 128; per head they would cost 40 times as much as the norm).  Lane i of a vector holds the elements 8 i.. and
-// R/2 + 8 i.. of the rotated part (halves: a pair stays in one lane), or 16 i..16 i + 15 (interleaved, or behind R).
+// (64 for a head of 128; per head they would cost 40 times as much as the norm).  A lane holds two pieces of 16 bytes (C elements) of a vector, at
+// C i of either half: of the rotated part's halves, so that a pair stays in one lane, of the rest's behind them, or, with pairs
+// side by side, of the vector's.  Neighbouring lanes load neighbouring pieces.
 template <typename E>
 __global__ void __launch_bounds__(256) bh_qk_norm_rotary_kernel(RotaryArgs a) {
+    constexpr int C = 16 / sizeof(E);
     extern __shared__ __attribute__((aligned(16))) float trig[];  // [tb][2][rot / 2]
     const int half = a.rot >> 1;
     const long long t0 = (long long)blockIdx.x * a.tb;
@@ -65,10 +85,16 @@ __global__ void __launch_bounds__(256) bh_qk_norm_rotary_kernel(RotaryArgs a) {
         trig[t * a.rot + half + j] = s;
     }
     __syncthreads();
-    const int heads = a.nq + a.nk, lpv = a.dim >> 4, lanes = 1 << a.lanes_log2;
-    const int i = threadIdx.x & (lanes - 1);
-    const bool live = i < lpv, turned = 16 * i < a.rot;
-    const int d0 = turned && !a.interleaved ? 8 * i : 16 * i, d1 = turned && !a.interleaved ? half + 8 * i : 16 * i + 8;
+    const int heads = a.nq + a.nk, lanes = 1 << a.lanes_log2;
+    const int i = threadIdx.x & (lanes - 1), in_first = half / C;  // lanes of the rotated part, where its halves are paired
+    const bool live = 2 * C * i < a.dim;
+    int d0, d1;
+    if (a.interleaved)
+        d0 = C * i, d1 = a.dim / 2 + C * i;
+    else if (i < in_first)
+        d0 = C * i, d1 = half + C * i;
+    else
+        d0 = a.rot + C * (i - in_first), d1 = a.rot + (a.dim - a.rot) / 2 + C * (i - in_first);
     for (int v = threadIdx.x >> a.lanes_log2; v < nt * heads; v += 256 >> a.lanes_log2) {
         const int t = v / heads, h = v - t * heads;
         const bool is_q = h < a.nq;
@@ -77,52 +103,51 @@ __global__ void __launch_bounds__(256) bh_qk_norm_rotary_kernel(RotaryArgs a) {
         E* dst = is_q ? static_cast<E*>(a.q_out) + (t0 + t) * a.qo_tok + h * a.qo_head
                       : static_cast<E*>(a.k_out) + (t0 + t) * a.ko_tok + (h - a.nq) * a.ko_head;
         const void* w = is_q ? a.qw : a.kw;
-        float x[8] = {}, y[8] = {};
+        float x[C] = {}, y[C] = {};
         if (live) {
-            bh_load8(src + d0, x);
-            bh_load8(src + d1, y);
+            load16<E, C>(src + d0, x);
+            load16<E, C>(src + d1, y);
         }
         if (w) {
             float ss = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ss += x[e] * x[e] + y[e] * y[e];
+            for (int e = 0; e < C; ++e) ss += x[e] * x[e] + y[e] * y[e];
             const float r = 1.0f / sqrtf(bh_group_sum(ss, lanes) / (float)a.dim + a.eps);
             if (live) {
-                float wx[8], wy[8];
-                weights8<E>(a, w, d0, wx);
-                weights8<E>(a, w, d1, wy);
+                float wx[C], wy[C];
+                weights<E, C>(a, w, d0, wx);
+                weights<E, C>(a, w, d1, wy);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
+                for (int e = 0; e < C; ++e) {
                     x[e] *= r * wx[e];
                     y[e] *= r * wy[e];
                 }
             }
         }
         if (!live) continue;
-        if (turned) {
-            float c[8], s[8];
-            bh_load8(&trig[t * a.rot + 8 * i], c);
-            bh_load8(&trig[t * a.rot + half + 8 * i], s);
-            if (a.interleaved) {
+        const float *cos_t = &trig[t * a.rot], *sin_t = cos_t + half;
+        if (a.interleaved) {
+            auto turn = [&](float(&z)[C], int d) {
+                if (d >= a.rot) return;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float u0 = x[2 * e], v0 = x[2 * e + 1], u1 = y[2 * e], v1 = y[2 * e + 1];
-                    x[2 * e] = u0 * c[e] - v0 * s[e];
-                    x[2 * e + 1] = v0 * c[e] + u0 * s[e];
-                    y[2 * e] = u1 * c[4 + e] - v1 * s[4 + e];
-                    y[2 * e + 1] = v1 * c[4 + e] + u1 * s[4 + e];
+                for (int e = 0; e < C / 2; ++e) {
+                    const float c = cos_t[d / 2 + e], s = sin_t[d / 2 + e], u = z[2 * e], p = z[2 * e + 1];
+                    z[2 * e] = u * c - p * s;
+                    z[2 * e + 1] = p * c + u * s;
                 }
-            } else {
+            };
+            turn(x, d0);
+            turn(y, d1);
+        } else if (i < in_first) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float u = x[e], p = y[e];
-                    x[e] = u * c[e] - p * s[e];
-                    y[e] = p * c[e] + u * s[e];
-                }
+            for (int e = 0; e < C; ++e) {
+                const float c = cos_t[d0 + e], s = sin_t[d0 + e], u = x[e], p = y[e];
+                x[e] = u * c - p * s;
+                y[e] = p * c + u * s;
             }
         }
-        bh_store8(dst + d0, x);
-        bh_store8(dst + d1, y);
+        store16<E, C>(dst + d0, x);
+        store16<E, C>(dst + d1, y);
     }
 }
 
@@ -266,10 +291,29 @@ struct cache_elem<BH_BF16> {
     typedef __bf16 type;
 };
 
-// grid.y: 0 keys, 1 values.
+// C codes of a piece, in C / 4 words.
+template <int CACHE, int C>
+__device__ __forceinline__ void store_codes(unsigned char* p, const float (&x)[C], float s, float inv, bool good) {
+    typedef unsigned words __attribute__((ext_vector_type(C / 4)));
+    words w;
+#pragma unroll
+    for (int i = 0; i < C / 4; ++i) {
+        unsigned c;
+        if constexpr (CACHE == BH_I8)
+            c = pack4_int8(x + 4 * i, s, inv);
+        else
+            c = pack4_e4m3(x + 4 * i, inv);
+        w[i] = good ? c : 0;
+    }
+    *reinterpret_cast<words*>(p) = w;
+}
+
+// grid.y: 0 keys, 1 values.  A lane has a piece of 16 bytes of the row (C elements) at C i of either half of the vector: neighbouring lanes
+// read and write next to each other on both sides (with one piece of 32 or 64 bytes a lane fp32 rows came at 3.8 TB/s).
 template <typename E, int CACHE>
 __global__ void __launch_bounds__(256) bh_kv_write_kernel(CacheArgs a) {
-    typedef typename cache_elem<CACHE>::type C;
+    typedef typename cache_elem<CACHE>::type T;
+    constexpr int C = 16 / sizeof(E);
     const int kv = blockIdx.y, lanes = 1 << a.lanes_log2, i = threadIdx.x & (lanes - 1);
     const long long v = ((long long)blockIdx.x * 256 + threadIdx.x) >> a.lanes_log2;
     if (v >= a.n_tokens * a.heads) return;  // whole groups
@@ -277,24 +321,25 @@ __global__ void __launch_bounds__(256) bh_kv_write_kernel(CacheArgs a) {
     const int h = (int)(v - t * a.heads);
     const long long slot = a.slots[t];
     if (slot < 0 || slot >= a.n_slots) return;
-    const E* src = static_cast<const E*>(a.src[kv]) + t * a.tok[kv] + h * a.head[kv] + 16 * i;
+    const int d0 = C * i, d1 = a.dim / 2 + C * i;
+    const E* src = static_cast<const E*>(a.src[kv]) + t * a.tok[kv] + h * a.head[kv];
     const long long at = vector_of(a, slot, h);
-    C* dst = static_cast<C*>(a.codes[kv]) + at * a.dim + 16 * i;
-    const bool live = 16 * i < a.dim;
-    float x[8] = {}, y[8] = {};
+    T* dst = static_cast<T*>(a.codes[kv]) + at * a.dim;
+    const bool live = 2 * C * i < a.dim;
+    float x[C] = {}, y[C] = {};
     if (live) {
-        bh_load8(src, x);
-        bh_load8(src + 8, y);
+        load16<E, C>(src + d0, x);
+        load16<E, C>(src + d1, y);
     }
     if constexpr (CACHE == BH_F16 || CACHE == BH_BF16) {
         if (live) {
-            bh_store8(dst, x);
-            bh_store8(dst + 8, y);
+            store16<T, C>(dst + d0, x);
+            store16<T, C>(dst + d1, y);
         }
     } else {
         unsigned most = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < C; ++e) {
             const unsigned p = __float_as_uint(x[e]) & 0x7fffffffu, q = __float_as_uint(y[e]) & 0x7fffffffu;
             most = most > p ? most : p;
             most = most > q ? most : q;
@@ -302,15 +347,9 @@ __global__ void __launch_bounds__(256) bh_kv_write_kernel(CacheArgs a) {
         const float s = scale_of<CACHE>(bh_group_umax(most, lanes));
         if (i == 0) a.scale[kv][at] = s;
         if (!live) return;
-        uint4 w = {0, 0, 0, 0};
-        if (s == s) {
-            const float inv = 1.0f / s;
-            if constexpr (CACHE == BH_I8)
-                w = {pack4_int8(x, s, inv), pack4_int8(x + 4, s, inv), pack4_int8(y, s, inv), pack4_int8(y + 4, s, inv)};
-            else
-                w = {pack4_e4m3(x, inv), pack4_e4m3(x + 4, inv), pack4_e4m3(y, inv), pack4_e4m3(y + 4, inv)};
-        }
-        *reinterpret_cast<uint4*>(dst) = w;
+        const float inv = 1.0f / s;
+        store_codes<CACHE, C>(dst + d0, x, s, inv, s == s);
+        store_codes<CACHE, C>(dst + d1, y, s, inv, s == s);
     }
 }
 
@@ -357,35 +396,46 @@ __global__ void __launch_bounds__(256) bh_kv_write_any_kernel(CacheArgs a) {
     }
 }
 
+template <int CACHE, int C>
+__device__ __forceinline__ void load_codes(const unsigned char* p, float s, float (&x)[C]) {
+    typedef unsigned words __attribute__((ext_vector_type(C / 4)));
+    const words w = *reinterpret_cast<const words*>(p);
+#pragma unroll
+    for (int i = 0; i < C / 4; ++i) {
+        if constexpr (CACHE == BH_I8)
+            unpack4_int8(w[i], s, x + 4 * i);
+        else
+            unpack4_e4m3(w[i], s, x + 4 * i);
+    }
+}
+
 template <typename E, int CACHE>
 __global__ void __launch_bounds__(256) bh_kv_read_kernel(CacheArgs a) {
-    typedef typename cache_elem<CACHE>::type C;
+    typedef typename cache_elem<CACHE>::type T;
+    constexpr int C = 16 / sizeof(E);
     const int kv = blockIdx.y, lanes = 1 << a.lanes_log2, i = threadIdx.x & (lanes - 1);
     const long long v = ((long long)blockIdx.x * 256 + threadIdx.x) >> a.lanes_log2;
-    if (v >= a.n_tokens * a.heads || 16 * i >= a.dim) return;
+    if (v >= a.n_tokens * a.heads || 2 * C * i >= a.dim) return;
     const long long t = v / a.heads;
     const int h = (int)(v - t * a.heads);
     const long long slot = a.slots[t];
-    E* dst = static_cast<E*>(a.dst[kv]) + t * a.tok[kv] + h * a.head[kv] + 16 * i;
-    float x[8] = {}, y[8] = {};
+    const int d0 = C * i, d1 = a.dim / 2 + C * i;
+    E* dst = static_cast<E*>(a.dst[kv]) + t * a.tok[kv] + h * a.head[kv];
+    float x[C] = {}, y[C] = {};
     if (slot >= 0 && slot < a.n_slots) {
         const long long at = vector_of(a, slot, h);
-        const C* src = static_cast<const C*>(a.codes[kv]) + at * a.dim + 16 * i;
+        const T* src = static_cast<const T*>(a.codes[kv]) + at * a.dim;
         if constexpr (CACHE == BH_F16 || CACHE == BH_BF16) {
-            bh_load8(src, x);
-            bh_load8(src + 8, y);
+            load16<T, C>(src + d0, x);
+            load16<T, C>(src + d1, y);
         } else {
-            const uint4 w = *reinterpret_cast<const uint4*>(src);
             const float s = a.scale[kv][at];
-            if constexpr (CACHE == BH_I8) {
-                unpack4_int8(w.x, s, x), unpack4_int8(w.y, s, x + 4), unpack4_int8(w.z, s, y), unpack4_int8(w.w, s, y + 4);
-            } else {
-                unpack4_e4m3(w.x, s, x), unpack4_e4m3(w.y, s, x + 4), unpack4_e4m3(w.z, s, y), unpack4_e4m3(w.w, s, y + 4);
-            }
+            load_codes<CACHE, C>(src + d0, s, x);
+            load_codes<CACHE, C>(src + d1, s, y);
         }
     }
-    bh_store8(dst, x);
-    bh_store8(dst + 8, y);
+    store16<E, C>(dst + d0, x);
+    store16<E, C>(dst + d1, y);
 }
 
 template <typename E, int CACHE>
@@ -460,7 +510,7 @@ int cache_call(bool write, const void* const (&x)[2], const long long (&tok)[2],
     if (scaled && (!scale[0] || !scale[1])) return bh_fail(BH_EINVAL, "an 8-bit cache needs the scales of keys and values");
     CacheArgs a{};
     const long long per16 = 16 / (long long)bh_dtype_size(dtype);
-    bool wide = head_dim % 16 == 0;
+    bool wide = head_dim % (2 * per16) == 0;
     for (int kv = 0; kv < 2; ++kv) {
         a.src[kv] = x[kv];
         a.dst[kv] = const_cast<void*>(x[kv]);
@@ -476,7 +526,7 @@ int cache_call(bool write, const void* const (&x)[2], const long long (&tok)[2],
     a.heads = n_heads;
     a.dim = head_dim;
     a.page_log2 = bh_ceil_log2(page_size);
-    a.lanes_log2 = bh_ceil_log2((head_dim + 15) / 16);
+    a.lanes_log2 = wide ? bh_ceil_log2((int)(head_dim / (2 * per16))) : 0;
     if (n_tokens > (1ll << 40) / n_heads || (n_tokens * n_heads) >> 28) return bh_fail(BH_EUNSUPPORTED, "more than 2^28 head vectors in one call");
     if (dtype == BH_F16)
         launch_cache_of<_Float16>(cache_dtype, a, write, wide, st);
@@ -517,7 +567,7 @@ int bh_op_qk_norm_rotary(const void* q, int64_t q_tok, int64_t q_head, void* q_o
     if (n_tokens == 0) return BH_OK;
     if (!q || !q_out || !k || !k_out || (rotary_dim && (!positions || !inv_freq))) return bh_fail(BH_EINVAL, "null buffer");
     const long long per16 = 16 / (long long)bh_dtype_size(dtype);
-    const bool wide = head_dim % 16 == 0 && rotary_dim % 16 == 0 && bh_aligned16(q) && bh_aligned16(k) && bh_aligned16(q_out) &&
+    const bool wide = head_dim % (2 * per16) == 0 && rotary_dim % (2 * per16) == 0 && bh_aligned16(q) && bh_aligned16(k) && bh_aligned16(q_out) &&
                       bh_aligned16(k_out) && bh_aligned16(q_weight) && bh_aligned16(k_weight) &&
                       (q_tok | q_head | qo_tok | qo_head | k_tok | k_head | ko_tok | ko_head) % per16 == 0;
     RotaryArgs a{};
@@ -528,7 +578,7 @@ int bh_op_qk_norm_rotary(const void* q, int64_t q_tok, int64_t q_head, void* q_o
     a.pos = positions, a.pos64 = positions_i64 != 0, a.inv_freq = inv_freq;
     a.n_tokens = n_tokens, a.nq = n_q_heads, a.nk = n_k_heads, a.dim = head_dim, a.rot = rotary_dim;
     a.w32 = weight_dtype == BH_F32, a.interleaved = interleaved != 0, a.eps = eps;
-    a.lanes_log2 = bh_ceil_log2((head_dim + 15) / 16);
+    a.lanes_log2 = wide ? bh_ceil_log2((int)(head_dim / (2 * per16))) : 0;
     // tokens of a workgroup: enough for two steps of its 256 threads where a token has few heads; the sines stay within 16 KiB of LDS
     const int lanes = (n_q_heads + n_k_heads) << a.lanes_log2;
     a.tb = lanes >= 512 ? 1 : 512 / lanes;

@@ -37,35 +37,39 @@ def _fail(message):
     raise ValueError(message)
 
 
-def _same_device(first, **others):
-    """Every tensor on one GPU, and none that waits for a gradient; -> that device."""
-    device = first.device
-    if device.type != "cuda":
-        _fail(f"tensors must be on the GPU, got one on {device}")
+def _one_device(names, *tensors):
+    """Every tensor (None: not given) on one GPU, and none that waits for a gradient; -> that GPU's index.  names: theirs, for a refusal."""
+    index = tensors[0].get_device()
     grad = torch.is_grad_enabled()
-    if grad and first.requires_grad:
-        _fail("no backward pass here: call under torch.no_grad()")
-    for name, t in others.items():
-        if t is not None:
-            if t.device != device:
-                _fail(f"{name} is on {t.device}, expected {device}")
-            if grad and t.requires_grad:
-                _fail(f"{name} requires a gradient and there is no backward pass here: call under torch.no_grad()")
-    if device.index not in _ready:
-        with torch.cuda.device(device):
-            _lib.init(device.index)  # once per device: is it a gfx950 part
-        _ready.add(device.index)
-    return device
+    for t in tensors:
+        if t is not None and (t.get_device() != index or (grad and t.requires_grad)):
+            for name, t in zip(names.split(), tensors):
+                if t is not None and t.get_device() != index:
+                    _fail(f"{name} is on {t.device}, expected {tensors[0].device}")
+                if t is not None and grad and t.requires_grad:
+                    _fail(f"{name} requires a gradient and there is no backward pass here: call under torch.no_grad()")
+    if index < 0:
+        _fail(f"tensors must be on the GPU, got them on {tensors[0].device}")
+    if index not in _ready:
+        with torch.cuda.device(index):
+            _lib.init(index)  # once per device: is it a gfx950 part
+        _ready.add(index)
+    return index
 
 
-def _call(device, fn, *args):
-    """fn(*args, stream) with the tensors' device as the current one, on its current stream."""
-    stream = _stream(device.index)
-    if torch.cuda.current_device() == device.index:
-        _lib.check(fn(*args, stream))
+def _call(index, fn, *args):
+    """fn(*args, stream) with GPU `index` as the current device, on its current stream."""
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _stream(index))
     else:
-        with torch.cuda.device(device):
-            _lib.check(fn(*args, stream))
+        with torch.cuda.device(index):
+            rc = fn(*args, _stream(index))
+    if rc:
+        _lib.check(rc)
+
+
+def _empty_like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _rows(name, t, heads=None, dim=None):
@@ -148,8 +152,8 @@ def qk_norm_rotary(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=
         _distinct("q", q)
         _distinct("k", k)
         _apart(q, k)
-    device = _same_device(q, k=k, positions=positions, inv_freq=inv_freq, q_weight=q_weight, k_weight=k_weight)
-    qo, ko = (q, k) if inplace else (q.new_empty(q.shape), k.new_empty(k.shape))
+    device = _one_device("q k positions inv_freq q_weight k_weight", q, k, positions, inv_freq, q_weight, k_weight)
+    qo, ko = (q, k) if inplace else (_empty_like(q), _empty_like(k))
     _call(device, _lib.lib().bh_op_qk_norm_rotary, q.data_ptr(), q.stride(0), q.stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1),
           k.data_ptr(), k.stride(0), k.stride(1), ko.data_ptr(), ko.stride(0), ko.stride(1), _FLOATS[q.dtype], tokens, nq, k.shape[1], dim,
           2 * inv_freq.numel(), positions.data_ptr(), int(positions.dtype == torch.int64), inv_freq.data_ptr(),
@@ -206,7 +210,7 @@ def kv_cache_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
         _fail("v must have k's shape and type")
     if not (slots.shape == (k.shape[0],) and slots.dtype == torch.int64 and slots.is_contiguous()):
         _fail(f"slots must be contiguous int64 [{k.shape[0]}]")
-    device = _same_device(k, v=v, slots=slots, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale)
+    device = _one_device("k v slots k_cache v_cache k_scale v_scale", k, v, slots, k_cache, v_cache, k_scale, v_scale)
     _call(device, _lib.lib().bh_op_kv_write, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _FLOATS[k.dtype],
           slots.data_ptr(), k.shape[0], heads, dim, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), _CACHES[k_cache.dtype],
           pages, page)
@@ -220,8 +224,9 @@ def kv_cache_read(slots, k_cache, v_cache, k_scale=None, v_scale=None, dtype=tor
         _fail(f"dtype must be float16, bfloat16 or float32, got {dtype}")
     if not (slots.dim() == 1 and slots.dtype == torch.int64 and slots.is_contiguous()):
         _fail("slots must be contiguous int64 [tokens]")
-    device = _same_device(slots, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale)
-    k, v = (torch.empty((slots.shape[0], heads, dim), dtype=dtype, device=device) for _ in range(2))
+    device = _one_device("slots k_cache v_cache k_scale v_scale", slots, k_cache, v_cache, k_scale, v_scale)
+    k = slots.new_empty((slots.shape[0], heads, dim), dtype=dtype)
+    v = torch.empty_like(k)
     _call(device, _lib.lib().bh_op_kv_read, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _FLOATS[dtype],
           slots.data_ptr(), slots.shape[0], heads, dim, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale),
           _CACHES[k_cache.dtype], pages, page)
@@ -254,18 +259,18 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, scale=None, k_sca
     if alibi_slopes is not None:
         if not (alibi_slopes.shape == (nq,) and alibi_slopes.dtype == torch.float32 and alibi_slopes.is_contiguous()):
             _fail(f"alibi_slopes must be contiguous float32 [{nq}]")
-    device = _same_device(q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, lengths=lengths, k_scale=k_scale, v_scale=v_scale,
-                          alibi_slopes=alibi_slopes)
+    device = _one_device("q k_cache v_cache block_table lengths k_scale v_scale alibi_slopes", q, k_cache, v_cache, block_table, lengths, k_scale,
+                         v_scale, alibi_slopes)
     if q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8:
         q = q.contiguous()
     lib, width = _lib.lib(), block_table.shape[1]
     need = lib.bh_op_paged_attention_workspace(batch, nq, heads, dim, page, width, int(window))
     if need < 0:
         _lib.check(need)
-    out = q.new_empty((batch, nq, dim))
-    lse = torch.empty((batch, nq), dtype=torch.float32, device=device) if return_lse else None
+    out = _empty_like(q)
+    lse = q.new_empty((batch, nq), dtype=torch.float32) if return_lse else None
     # (made anew for each call: two calls at once, or two captured graphs, must not share one)
-    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    work = lengths.new_empty(need, dtype=torch.uint8) if need else None
     _call(device, lib.bh_op_paged_attention, q.data_ptr(), q.stride(0), q.stride(1), _FLOATS[q.dtype], k_cache.data_ptr(), v_cache.data_ptr(),
           _ptr(k_scale), _ptr(v_scale), _CACHES[k_cache.dtype], pages, page, block_table.data_ptr(), block_table.stride(0), width,
           lengths.data_ptr(), batch, nq, heads, dim, float(dim ** -0.5 if scale is None else scale), float(softcap), int(window),
@@ -288,7 +293,7 @@ def token_logprobs(logits, targets, top=0):
         _fail("logits' rows must be dense and not empty")
     if not (targets.dtype == torch.int64 and targets.dim() in (1, 2) and targets.shape[0] == rows and targets.is_contiguous()):
         _fail(f"targets must be contiguous int64 [{rows}] or [{rows}, given]")
-    device = _same_device(logits, targets=targets)
+    device = _one_device("logits targets", logits, targets)
     if rows > 1 and logits.stride(0) < vocab:
         logits = logits.contiguous()
     lib, top = _lib.lib(), int(top)
@@ -299,7 +304,7 @@ def token_logprobs(logits, targets, top=0):
     entropy = logits.new_empty((rows,), dtype=torch.float32)
     top_logprobs = logits.new_empty((rows, top), dtype=torch.float32)
     top_ids = targets.new_empty((rows, top))
-    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    work = targets.new_empty(need, dtype=torch.uint8) if need else None
     _call(device, lib.bh_op_token_logprobs, logits.data_ptr(), logits.stride(0), _FLOATS[logits.dtype], rows, vocab, targets.data_ptr(),
           1 if targets.dim() == 1 else targets.shape[1], top, logprobs.data_ptr(), entropy.data_ptr(), top_logprobs.data_ptr(),
           top_ids.data_ptr(), _ptr(work), need)

@@ -159,11 +159,11 @@ def test_older_entry_points_still_refuse_the_new_types():
 
 def test_a_gradient_is_refused_while_it_is_recorded():
     from bergen_amd import decoding
-
-    class OnGpu:  # what the check looks at, without a device
-        requires_grad, device = True, torch.device("cuda", 0)
-    with pytest.raises(ValueError, match="no backward pass"):
-        decoding._same_device(OnGpu())
+    leaf = torch.zeros(2, requires_grad=True)
+    with pytest.raises(ValueError, match="k requires a gradient"):
+        decoding._one_device("q k", torch.zeros(2), leaf)
+    with torch.no_grad(), pytest.raises(ValueError, match="must be on the GPU"):
+        decoding._one_device("q k", torch.zeros(2), leaf)
 
 
 def test_rotary_frequencies():
