@@ -531,7 +531,9 @@ int cache_call(bool write, const void* const (&x)[2], const long long (&tok)[2],
     a.dim = head_dim;
     a.page_log2 = bh_ceil_log2(page_size);
     a.lanes_log2 = wide ? bh_ceil_log2((int)(head_dim / (2 * per16))) : 0;
-    if (n_tokens > (1ll << 40) / n_heads || (n_tokens * n_heads) >> 28) return bh_fail(BH_EUNSUPPORTED, "more than 2^28 head vectors in one call");
+    // (2^24 workgroups of 256 threads are as many as a grid's first dimension can have)
+    if (n_tokens > (1ll << 40) / n_heads || ((n_tokens * n_heads) << (wide ? a.lanes_log2 : 6)) >> 32)
+        return bh_fail(BH_EUNSUPPORTED, "too many head vectors in one call");
     if (dtype == BH_F16)
         launch_cache_of<_Float16>(cache_dtype, a, write, wide, st);
     else if (dtype == BH_BF16)
@@ -586,6 +588,7 @@ int bh_op_qk_norm_rotary(const void* q, int64_t q_tok, int64_t q_head, void* q_o
     // tokens of a workgroup: enough for two steps of its 256 threads where a token has few heads; the sines stay within 16 KiB of LDS
     const int lanes = (n_q_heads + n_k_heads) << a.lanes_log2;
     a.tb = lanes >= 512 ? 1 : 512 / lanes;
+    if (n_tokens / (wide ? a.tb : 1) >= (1 << 24) - 1) return bh_fail(BH_EUNSUPPORTED, "too many tokens in one call");
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (dtype == BH_F16)
         launch_rotary<_Float16>(a, wide, st);

@@ -15,6 +15,7 @@
 namespace {
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr float FAR = 1e37f;
 constexpr int MAX_TOP = 64, WAVES = 4, THREADS = 64 * WAVES;
 
 struct LogprobArgs {
@@ -189,6 +190,7 @@ __global__ void __launch_bounds__(THREADS, 4) bh_token_logprobs_kernel(LogprobAr
     Seen s{-INFINITY, 0.f, 0.f, false};  // m: the wave's; rest, first: the lane's
     float m2 = 0.f;                      // m log2(e), rounded (0 while there is nothing but -inf): what the exponents are taken from, and
     float off2 = 0.f;                    // what the rounding left of it: 2^off2 is the maximum's own weight, put right at the end
+    bool huge = false;                   // m log2(e) is beyond fp32 (a row of nothing but the type's lowest value): exponents from m itself
     u64 best = 0, bar = 0;               // the lane's key of the wave's list; the k-th key: what is not above it cannot be among the k
     float bar_x = __uint_as_float(0x7fc00000u);  // its value; a NaN lets everything through
 
@@ -288,7 +290,7 @@ __global__ void __launch_bounds__(THREADS, 4) bh_token_logprobs_kernel(LogprobAr
         if (__any(step_most > s.m)) {  // a new maximum: a few times in a row
             const float top_x = wave_max(step_most);
             if (s.m > -INFINITY && top_x < INFINITY) {
-                const float by = m2 - __fmul_rn(top_x, LOG2E), f = __builtin_amdgcn_exp2f(by);
+                const float by = huge || fabsf(top_x) > FAR ? (s.m - top_x) * LOG2E : m2 - __fmul_rn(top_x, LOG2E), f = __builtin_amdgcn_exp2f(by);
                 if (lane == 0) {  // the old maximum is one of many now
                     const float own = __builtin_amdgcn_exp2f(off2);
                     s.rest += own;
@@ -298,8 +300,9 @@ __global__ void __launch_bounds__(THREADS, 4) bh_token_logprobs_kernel(LogprobAr
                 s.rest *= f;
             }
             s.m = top_x;
-            m2 = __fmul_rn(top_x, LOG2E);
-            off2 = top_x < INFINITY ? fmaf(top_x, LOG2E, -m2) : 0.f;
+            huge = fabsf(top_x) > FAR;
+            m2 = huge ? 0.f : __fmul_rn(top_x, LOG2E);
+            off2 = huge ? 0.f : fmaf(top_x, LOG2E, -m2);
             // its own 1 is left out: one element that equals it, of one lane
             bool mine = lane == __ffsll((unsigned long long)__ballot(step_most == top_x)) - 1;
 #pragma unroll
@@ -311,6 +314,10 @@ __global__ void __launch_bounds__(THREADS, 4) bh_token_logprobs_kernel(LogprobAr
                         mine = false;
                     }
             if (top_x == INFINITY) s.rest = __uint_as_float(0x7fc00000u);
+        }
+        if (__any(huge)) {
+#pragma unroll
+            for (int b = 0; b < U * N; ++b) xs[b] -= s.m;
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -425,7 +432,7 @@ int bh_op_token_logprobs(const void* logits, int64_t row_stride, int32_t dtype, 
     const int64_t need = a.parts > 1 ? n_rows * a.parts * (16 + 8 * (int64_t)top) : 0;
     if (need && (!workspace || workspace_bytes < need || !bh_aligned16(workspace)))
         return bh_fail(BH_EINVAL, "workspace of %lld bytes, 16-byte aligned, needed: %lld given", (long long)need, (long long)workspace_bytes);
-    if (n_rows * a.parts > 0x7fffffffll) return bh_fail(BH_EUNSUPPORTED, "too many rows");
+    if (n_rows * a.parts >= 1 << 24) return bh_fail(BH_EUNSUPPORTED, "too many rows");
     a.x = logits;
     a.stride = row_stride;
     a.targets = reinterpret_cast<const long long*>(targets);

@@ -159,6 +159,8 @@ def qk_norm_rotary(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=
           2 * inv_freq.numel(), positions.data_ptr(), int(positions.dtype == torch.int64), inv_freq.data_ptr(),
           q_weight.data_ptr() if q_weight is not None else None, k_weight.data_ptr() if k_weight is not None else None,
           _FLOATS[wtype or q.dtype], float(eps), int(bool(interleaved)))
+    if inplace:
+        torch.autograd.graph.increment_version((q, k))
     return qo, ko
 
 
@@ -210,6 +212,8 @@ def kv_cache_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
         _fail("v must have k's shape and type")
     if not (slots.shape == (k.shape[0],) and slots.dtype == torch.int64 and slots.is_contiguous()):
         _fail(f"slots must be contiguous int64 [{k.shape[0]}]")
+    if k_cache.data_ptr() == v_cache.data_ptr() and k_cache.numel():
+        _fail("k_cache and v_cache are the same memory")
     device = _one_device("k v slots k_cache v_cache k_scale v_scale", k, v, slots, k_cache, v_cache, k_scale, v_scale)
     _call(device, _lib.lib().bh_op_kv_write, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _FLOATS[k.dtype],
           slots.data_ptr(), k.shape[0], heads, dim, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), _CACHES[k_cache.dtype],
@@ -259,6 +263,8 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, scale=None, k_sca
     if alibi_slopes is not None:
         if not (alibi_slopes.shape == (nq,) and alibi_slopes.dtype == torch.float32 and alibi_slopes.is_contiguous()):
             _fail(f"alibi_slopes must be contiguous float32 [{nq}]")
+    if not 0 <= window < 1 << 31:
+        _fail(f"window must be 0 or a count of tokens, got {window}")
     device = _one_device("q k_cache v_cache block_table lengths k_scale v_scale alibi_slopes", q, k_cache, v_cache, block_table, lengths, k_scale,
                          v_scale, alibi_slopes)
     if q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8:
@@ -293,6 +299,8 @@ def token_logprobs(logits, targets, top=0):
         _fail("logits' rows must be dense and not empty")
     if not (targets.dtype == torch.int64 and targets.dim() in (1, 2) and targets.shape[0] == rows and targets.is_contiguous()):
         _fail(f"targets must be contiguous int64 [{rows}] or [{rows}, given]")
+    if not 0 <= top <= vocab:
+        _fail(f"top {top} of {vocab} tokens")
     device = _one_device("logits targets", logits, targets)
     if rows > 1 and logits.stride(0) < vocab:
         logits = logits.contiguous()

@@ -70,6 +70,8 @@ def test_cache_refusals():
                           (dict(k_cache=base["k_cache"].transpose(0, 1), v_cache=base["v_cache"].transpose(0, 1)), "contiguous"),
                           (dict(), "must be on the GPU")]:
         _refused(match, bergen_amd.kv_cache_write, **{**base, **change})
+    same = _cache_args()
+    _refused("the same memory", bergen_amd.kv_cache_write, k, k, slots, **dict(same, v_cache=same["k_cache"]))
     half = dict(_cache_args(torch.float16), k_scale=torch.zeros(2, 3, 16))
     _refused("has no scales", bergen_amd.kv_cache_read, slots, **half)
     _refused("dtype must be", bergen_amd.kv_cache_read, slots, **_cache_args(), dtype=torch.int8)
@@ -83,7 +85,7 @@ def test_attention_refusals():
     for change, match in [(dict(q=torch.zeros(2, 6, 32)), "q must be float16 or bfloat16"), (dict(q=torch.zeros(2, 6, 48, dtype=torch.bfloat16)), "q has shape"),
                           (dict(block_table=torch.zeros(3, 4, dtype=torch.int32)), "block_table"), (dict(block_table=torch.zeros(2, 4).long()), "block_table"),
                           (dict(lengths=torch.zeros(2)), "lengths"), (dict(lengths=torch.zeros(3, dtype=torch.int32)), "lengths"),
-                          (dict(alibi_slopes=torch.zeros(3)), "alibi_slopes"), (_cache_args(torch.float16), "the cache must be"),
+                          (dict(window=-1), "window"), (dict(window=1 << 32), "window"), (dict(alibi_slopes=torch.zeros(3)), "alibi_slopes"), (_cache_args(torch.float16), "the cache must be"),
                           (dict(), "must be on the GPU")]:
         _refused(match, bergen_amd.paged_attention, **{**base, **change})
 
@@ -91,7 +93,8 @@ def test_attention_refusals():
 def test_logprobs_refusals():
     x, t = torch.zeros(2, 9), torch.zeros(2, dtype=torch.int64)
     for a, match in [((x.double(), t), "logits must be"), ((x[0], t), "logits must be"), ((x[:, :0], t), "not empty"), ((x.t(), t), "dense"),
-                     ((x, t.int()), "targets"), ((x, t[:1]), "targets"), ((x, t), "must be on the GPU")]:
+                     ((x, t.int()), "targets"), ((x, t[:1]), "targets"), ((x, t, 10), "top 10 of 9"),
+                     ((x, t, -1), "top -1"), ((x, t, 1 << 32), "top"), ((x, t), "must be on the GPU")]:
         _refused(match, bergen_amd.token_logprobs, *a)
 
 
@@ -105,7 +108,7 @@ def test_refused_by_the_c_entry_points():
 
     for code, k in [(E, dict(dtype=I8)), (E, dict(dtype=9)), (E, dict(qw=P, wt=H)), (E, dict(tokens=-1)), (E, dict(nq=0)), (E, dict(eps=-1.0)),
                     (E, dict(eps=math.nan)), (U, dict(dim=257)), (U, dict(dim=0)), (E, dict(rot=66)), (E, dict(rot=63)), (E, dict(rot=-2)),
-                    (U, dict(tokens=1 << 31)), (E, dict(q=None)), (E, dict(pos=None)), (E, dict(inv=None))]:
+                    (U, dict(tokens=1 << 31)), (U, dict(tokens=1 << 30)), (U, dict(tokens=1 << 24, dim=63, rot=62)), (E, dict(q=None)), (E, dict(pos=None)), (E, dict(inv=None))]:
         assert rotary(**k) == code, k
         assert lib.bh_last_error(), k
     assert rotary(tokens=0) == _lib.BH_OK
@@ -116,7 +119,7 @@ def test_refused_by_the_c_entry_points():
     for fn in (lib.bh_op_kv_write, lib.bh_op_kv_read):
         for code, k in [(E, dict(dtype=I8)), (E, dict(cache=F)), (E, dict(cache=7)), (E, dict(tokens=-1)), (E, dict(heads=0)), (E, dict(pages=0)),
                         (U, dict(dim=257)), (U, dict(page=4)), (U, dict(page=24)), (U, dict(page=2048)), (E, dict(k=None)), (E, dict(slots=None)),
-                        (E, dict(scale=None)), (U, dict(tokens=1 << 40)), (U, dict(tokens=1 << 28))]:
+                        (E, dict(scale=None)), (U, dict(tokens=1 << 40)), (U, dict(tokens=1 << 30)), (U, dict(tokens=1 << 28, dim=63))]:
             assert write(fn=fn, **k) == code, k
         assert write(fn=fn, tokens=0) == _lib.BH_OK
 
@@ -143,7 +146,7 @@ def test_refused_by_the_c_entry_points():
     for code, k in [(E, dict(dtype=I8)), (E, dict(rows=-1)), (E, dict(vocab=0)), (E, dict(top=101)), (E, dict(top=-1)), (U, dict(top=65)), (E, dict(given=-1)),
                     (E, dict(stride=99)), (E, dict(x=None)), (E, dict(t=None)), (E, dict(ids=None)), (U, dict(vocab=(1 << 30) + 1, stride=1 << 31)),
                     (U, dict(rows=(1 << 24) + 1)), (E, dict(x=ctypes.c_void_p(4098))), (E, dict(vocab=100000, stride=100000, n=8)),
-                    (E, dict(vocab=100000, stride=100000, ws=None))]:
+                    (E, dict(vocab=100000, stride=100000, ws=None)), (U, dict(rows=1 << 24))]:
         assert logp(**k) == code, k
     assert logp(rows=0) == _lib.BH_OK
     assert lib.bh_op_token_logprobs_workspace(1, 100000, F, 5) > 0 and lib.bh_op_token_logprobs_workspace(100000, 1000, F, 5) == 0

@@ -57,7 +57,9 @@ def test_rotary_strides(dtype):
     qkv = randn(g, 9, 10, 64, dtype=dtype)
     rest = qkv[:, 8:].clone()
     check_rotary(qkv[:, :6], qkv[:, 6:8], pos, f, w, w)
+    before = qkv._version
     check_rotary(qkv[:, :6], qkv[:, 6:8], pos, f, w, w, inplace=True)
+    assert qkv._version > before                                # autograd is told
     assert torch.equal(qkv[:, 8:], rest)
     odd = randn(g, 9 * 10 * 65 + 1, dtype=dtype)[1:].view(9, 10, 65)
     check_rotary(odd[:, :6, :64], odd[:, 6:8, 1:], pos, f, w, w)
@@ -434,6 +436,29 @@ def test_logprobs_rows_and_ties(dtype):
     r = bergen_amd.token_logprobs(x, t, top=3)
     assert r.top_ids[0].tolist() == [0, 1, 2] and r.entropy[3] == 0 and (r.logprobs[3] == -math.inf).all()
     assert abs(float(r.entropy[0]) - math.log(n)) < 1e-5 and torch.isnan(r.logprobs[12]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+def test_logprobs_of_a_types_limits(dtype):
+    """The type's lowest value as a mask, in a whole row too (which is then uniform), its largest, its smallest, and a row of NaN alone."""
+    low, high, n = torch.finfo(dtype).min, torch.finfo(dtype).max, 5000
+    g = torch.Generator().manual_seed(3)
+    some = torch.randn(n, generator=g)
+    masked, above = some.clone(), some.clone()
+    masked[::3], above[4000] = low, high
+    late = torch.full((n,), low)
+    late[4999] = -5.0
+    rows = [torch.full((n,), low), masked, above, late, torch.full((n,), high), torch.full((n,), torch.finfo(dtype).tiny), torch.full((n,), math.nan)]
+    x = torch.stack(rows).to(dtype).cuda()
+    t = torch.tensor([0, 4000, 4999], device="cuda").expand(len(rows), 3).contiguous()
+    for top in (0, 5):
+        r = check_logprobs(x, t, top)
+    for i in (0, 4, 5):
+        assert abs(float(r.entropy[i]) - math.log(n)) < 1e-5 and torch.allclose(r.logprobs[i], torch.full((3,), -math.log(n), device="cuda"), atol=1e-5)
+    assert torch.isnan(r.logprobs[6]).all() and r.top_ids[6].tolist() == [0, 1, 2, 3, 4]
+    parts = torch.full((1, 70000), low, device="cuda", dtype=dtype)       # several parts of a row
+    parts[0, 69000] = low / 2
+    check_logprobs(parts, torch.tensor([69000], device="cuda"), 3)
 
 
 def test_entropy_of_a_nearly_certain_row():
