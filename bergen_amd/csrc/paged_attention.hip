@@ -44,7 +44,8 @@ struct PagedArgs {
     float* part_stats;  // [batch][hq][splits][2]: m log2(e), sum
     float* part_out;    // [batch][hq][splits][dim], not yet divided
     int batch, hq, hk, group, blocks, dim, n_pages, page_log2, table_width;
-    int splits, per_split;  // per_split: tokens, a multiple of WAVES * TILE
+    int splits, per_split;  // of a sequence at most; tokens of one, for the longest that the table allows
+    int work;               // batch times key heads (times blocks of 16 query heads), at most 256
     int window;
     float scale, softcap;
 };
@@ -68,6 +69,28 @@ template <typename T>
 __device__ __forceinline__ T streamed(const unsigned char* p) {
     typedef unsigned words __attribute__((ext_vector_type(sizeof(T) / 4)));
     return __builtin_bit_cast(T, __builtin_nontemporal_load(reinterpret_cast<const words*>(p)));
+}
+
+// A sequence's tokens that count, [start, len), and its splits: `per` tokens each from `first` on, the tile that start lies in.
+struct Range {
+    int start, len, first, per, live;
+};
+__device__ __forceinline__ Range range_of(const PagedArgs& a, int seq) {
+    Range r;
+    const long long most = (long long)a.table_width << a.page_log2;
+    r.len = a.lengths[seq];
+    r.len = r.len < 0 ? 0 : r.len > most ? (int)most : r.len;
+    r.start = a.window > 0 && r.len > a.window ? r.len - a.window : 0;
+    r.first = r.start & ~(TILE - 1);
+    // as many tokens as a sequence of its own length would get (a wide table says little of what is in use); longer ones where the splits run out
+    constexpr int STEP = WAVES * TILE;
+    const int tokens = r.len - r.first, share = (tokens + a.splits - 1) / a.splits;
+    const long long even = (long long)tokens * a.work / 256;
+    r.per = even < a.per_split ? (int)even : a.per_split;
+    r.per = ((r.per > share ? r.per : share) + STEP - 1) / STEP * STEP;
+    r.per = r.per < STEP ? STEP : r.per;
+    r.live = (tokens + r.per - 1) / r.per;
+    return r;
 }
 
 __device__ __forceinline__ float over_groups_max(float v) {  // over the 4 lanes with the same lane % 16
@@ -122,15 +145,11 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : DP == 64 ? 4 : EXA
     const int hq0 = hk * a.group + 16 * block;                       // the first of this workgroup's query heads
     const int heads = a.group - 16 * block < 16 ? a.group - 16 * block : 16;
 
-    int len = a.lengths[seq];
-    const long long most = (long long)a.table_width << a.page_log2;
-    len = len < 0 ? 0 : len > most ? (int)most : len;
-    const int start = a.window > 0 && len > a.window ? len - a.window : 0;
-    const int first = start & ~(TILE - 1);
-    const int live_splits = (len - first + a.per_split - 1) / a.per_split;
+    const Range range = range_of(a, seq);
+    const int len = range.len, start = range.start, live_splits = range.live;
     if (split >= live_splits && split > 0) return;
-    const int lo = first + split * a.per_split;
-    const int hi = lo + a.per_split < len ? lo + a.per_split : len;
+    const int lo = range.first + split * range.per;
+    const int hi = lo + range.per < len ? lo + range.per : len;
 
     // ---- the queries, operand B of S^T: lane (g, n) holds head n, dims as its key chunks
     const bool head_live = n < heads;
@@ -348,7 +367,9 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : DP == 64 ? 4 : EXA
                 for (int j = 0; j < NJ; ++j) o[j] *= fade;
             }
             if constexpr (SCALED) {
-                const float big = fmaxf(fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])), fmaxf(fmaxf(vs[4], vs[5]), fmaxf(vs[6], vs[7])));
+                float big = fabsf(vs[0]);
+#pragma unroll
+                for (int r = 1; r < 8; ++r) big = fmaxf(big, fabsf(vs[r]));
                 if (__any(big > v_top)) {
                     // the power of two at or above the largest scale of the wave's tokens so far
                     const unsigned b = __float_as_uint(over_groups_max(big));
@@ -487,11 +508,7 @@ __global__ void __launch_bounds__(256) bh_paged_attention_join_kernel(PagedArgs 
     __shared__ float sh[4];
     __shared__ floatx4 sh_out[256];
     const int head = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x;
-    int len = a.lengths[seq];
-    const long long most = (long long)a.table_width << a.page_log2;
-    len = len < 0 ? 0 : len > most ? (int)most : len;
-    const int start = a.window > 0 && len > a.window ? len - a.window : 0;
-    const int live = (len - (start & ~(TILE - 1)) + a.per_split - 1) / a.per_split;
+    const int live = range_of(a, seq).live;
     if (live <= 1) return;  // written by its only workgroup
     const long long at = (long long)seq * a.hq + head;
     const float* stats = a.part_stats + 2 * at * a.splits;
@@ -531,22 +548,23 @@ __global__ void __launch_bounds__(256) bh_paged_attention_join_kernel(PagedArgs 
     }
 }
 
-// How the cache's length is split, by the longest length that the table allows (the lengths themselves are on the device); a sequence uses
-// as many splits as its own length fills.  A CU takes about 30 GB/s whatever runs on it (700 tokens of one key head in one workgroup of 4
+// How the cache's length is split, by the longest length that the table allows (the lengths themselves are on the device); range_of does the same
+// again for each sequence's own.  A CU takes about 30 GB/s whatever runs on it (700 tokens of one key head in one workgroup of 4
 // waves or of 8: 12 us), so few sequences are spread over all 256 of them, down to 128 tokens a workgroup (one tile a wave: 6.7 us); beyond
 // that fewer, longer splits cost less (64 sequences, up to 8191 tokens: 194 / 187 / 192 us in splits of 512 / 1024 / 2048; a window of
 // 4096 on 444 heads: 41 / 43 / 53).  The join is a second launch of 3.7 us and more: none up to 768 tokens (8 heads, 700 tokens: 12.0 against 6.6 + 3.7
-// and a launch), nor up to 2048 where the sequences alone fill the chip (32 sequences, up to 2000 tokens: 43.4 against 45.4 + 4.6).
+// and a launch), nor up to 2048 where the sequences alone fill the chip (32 sequences, up to 2000 tokens: 43.4 against 45.4 + 4.6).  At most
+// 16384 workgroups, or 16 splits, however wide the table (65 thousand that find nothing to do take 20 us, and each split its workspace): a sequence
+// that is longer than that many splits takes longer ones.
 void split_length(int64_t batch, int64_t blocks, int64_t longest, int32_t window, int* splits, int* per_split) {
     if (window > 0 && window + TILE < longest) longest = window + TILE;  // (a window's start is rounded down to a tile)
     const int64_t work = batch * blocks, step = WAVES * TILE;
     int64_t per = (longest * work / 256 + step - 1) / step * step;
     per = per < step ? step : per > 1024 ? 1024 : per;
     if (longest <= 768 || (longest <= 2048 && work >= 256)) per = (longest + step - 1) / step * step;
-    if (longest > per * 4096) per = (longest / 4096 + step) / step * step;  // (the join holds the splits' weights in LDS)
     *per_split = (int)(per < step ? step : per);
-    const int64_t n = (longest + *per_split - 1) / *per_split;
-    *splits = (int)(n < 1 ? 1 : n);
+    int64_t n = (longest + *per_split - 1) / *per_split, most = work > 1024 ? 16 : work < 4 ? 4096 : 16384 / work;
+    *splits = (int)(n < 1 ? 1 : n < most ? n : most);
 }
 
 template <typename E, int CACHE, int DP, bool EXACT>
@@ -628,6 +646,7 @@ int bh_op_paged_attention(const void* q, int64_t q_seq, int64_t q_head, int32_t 
     a.table = table, a.table_stride = table_stride, a.lengths = lengths;
     a.part_out = static_cast<float*>(workspace);
     a.part_stats = a.part_out + parts * head_dim;
+    a.work = (int64_t)batch * n_k_heads * a.blocks < 256 ? batch * n_k_heads * a.blocks : 256;
     a.batch = batch, a.hq = n_q_heads, a.hk = n_k_heads, a.dim = head_dim, a.n_pages = (int)n_pages;
     a.page_log2 = bh_ceil_log2(page_size), a.table_width = n_pages ? table_width : 0;
     a.window = window, a.scale = scale, a.softcap = softcap;

@@ -367,6 +367,17 @@ def test_attention_far_into_a_cache():
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("cache", [BF, E4])
+def test_attention_with_a_wide_table(cache):
+    """A table far wider than most sequences need, and more splits wanted than there are: a long sequence takes longer ones."""
+    g = gen(12)
+    lengths = [33000] + [60] * 63 + [0, 16385]
+    pages = sum(-(-n // 8) for n in lengths)
+    c = made_cache(g, pages, 24, 8, 16, cache)
+    table = table_for(g, lengths, 8, pages, extra=12000)
+    check_attention(randn(g, len(lengths), 24, 16, dtype=BF), c, table, lengths)
+
+
 def test_attention_strides():
     g = gen(10)
     c = made_cache(g, 6, 2, 16, 64, BF)
