@@ -15,7 +15,6 @@ They take device tensors, ENQUEUE on the current stream of the tensors' device a
 be captured into a graph.  They run inference only: a tensor that requires a gradient is refused while gradients are recorded.
 """
 import collections
-import ctypes
 
 import torch
 
@@ -31,6 +30,10 @@ _ready = set()
 
 # the current stream's handle: current_stream() builds an object around it, which takes longer than the launch it is wanted for
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+# (likewise: the index without the question whether CUDA is initialised, which a tensor on the GPU has answered)
+_current = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _fail(message):
@@ -59,7 +62,7 @@ def _one_device(names, *tensors):
 
 def _call(index, fn, *args):
     """fn(*args, stream) with GPU `index` as the current device, on its current stream."""
-    if torch.cuda.current_device() == index:
+    if _current() == index:
         rc = fn(*args, _stream(index))
     else:
         with torch.cuda.device(index):
@@ -72,16 +75,21 @@ def _empty_like(t):
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
-def _rows(name, t, heads=None, dim=None):
-    """[tokens, heads, dim] with the last dimension dense."""
+def _rows(name, t):
+    """[tokens, heads, dim] with the last dimension dense -> its sizes, the strides of the first two, its address."""
     if t.dim() != 3:
         _fail(f"{name} must be [tokens, heads, dim], got {tuple(t.shape)}")
     if t.dtype not in _FLOATS:
         _fail(f"{name} must be float16, bfloat16 or float32, got {t.dtype}")
-    if not ((heads is None or t.shape[1] == heads) and (dim is None or t.shape[2] == dim)):
-        _fail(f"{name} has shape {tuple(t.shape)}")
-    if not (t.shape[2] <= 1 or t.stride(2) == 1):
+    tokens, heads, dim = t.shape
+    by_token, by_head, dense = t.stride()
+    if dense != 1 and dim > 1:
         _fail(f"{name}'s last dimension must be dense")
+    return tokens, heads, dim, by_token, by_head, t.data_ptr()
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
 
 
 def _distinct(name, t):
@@ -119,6 +127,12 @@ def rotary_frequencies(rotary_dim, theta=10000.0, scale=1.0, device="cuda"):
     return float(scale) * float(theta) ** (-j / max(1, rotary_dim))
 
 
+def _weight(name, w, dim, dtype):
+    if w.dim() != 1 or w.shape[0] != dim or not (w.dtype == dtype or w.dtype == torch.float32) or not w.is_contiguous():
+        _fail(f"{name} must be contiguous [{dim}], {dtype} or float32")
+    return w.dtype
+
+
 def qk_norm_rotary(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, inplace=False):
     """RMS norm of each head of q [tokens, n_q, dim] and k [tokens, n_k, dim], then rotary positions, in one pass -> (q, k).
 
@@ -127,38 +141,36 @@ def qk_norm_rotary(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=
     or float32; None: that side is not normalised.  q and k are float16, bfloat16 or float32, any strides with a dense last
     dimension (slices of one projection).  inplace: into q and k themselves.
     """
-    _rows("q", q)
-    _rows("k", k, dim=q.shape[2])
-    tokens, nq, dim = q.shape
-    if not (k.dtype == q.dtype and k.shape[0] == tokens):
-        _fail(f"k must be [{tokens}, heads, {dim}] {q.dtype}, got {tuple(k.shape)} {k.dtype}")
-    if not (positions.shape == (tokens,) and positions.dtype in (torch.int32, torch.int64)):
+    tokens, nq, dim, q0, q1, qp = _rows("q", q)
+    tokens_k, nk, dim_k, k0, k1, kp = _rows("k", k)
+    dtype = q.dtype
+    if k.dtype != dtype or tokens_k != tokens or dim_k != dim:
+        _fail(f"k must be [{tokens}, heads, {dim}] {dtype}, got {tuple(k.shape)} {k.dtype}")
+    wide = positions.dtype == torch.int64
+    if not (wide or positions.dtype == torch.int32) or positions.dim() != 1 or positions.shape[0] != tokens:
         _fail(f"positions must be int32 or int64 [{tokens}]")
-    if not (inv_freq.dim() == 1 and inv_freq.dtype == torch.float64 and 2 * inv_freq.numel() <= dim):
+    rotary = 2 * inv_freq.numel()
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or rotary > dim:
         _fail(f"inv_freq must be float64 [rotary_dim / 2], rotary_dim at most {dim}")
-    wtype = None
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None:
-            if not (w.shape == (dim,) and w.dtype in (q.dtype, torch.float32)):
-                _fail(f"{name} must be [{dim}], {q.dtype} or float32")
-            if not (wtype in (None, w.dtype)):
-                _fail("q_weight and k_weight must have one type")
-            if not w.is_contiguous():
-                _fail(f"{name} must be contiguous")
-            wtype = w.dtype
     if not (positions.is_contiguous() and inv_freq.is_contiguous()):
         _fail("positions and inv_freq must be contiguous")
+    wtype = _weight("q_weight", q_weight, dim, dtype) if q_weight is not None else None
+    if k_weight is not None:
+        was, wtype = wtype, _weight("k_weight", k_weight, dim, dtype)
+        if was not in (None, wtype):
+            _fail("q_weight and k_weight must have one type")
     if inplace:
         _distinct("q", q)
         _distinct("k", k)
         _apart(q, k)
     device = _one_device("q k positions inv_freq q_weight k_weight", q, k, positions, inv_freq, q_weight, k_weight)
-    qo, ko = (q, k) if inplace else (_empty_like(q), _empty_like(k))
-    _call(device, _lib.lib().bh_op_qk_norm_rotary, q.data_ptr(), q.stride(0), q.stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1),
-          k.data_ptr(), k.stride(0), k.stride(1), ko.data_ptr(), ko.stride(0), ko.stride(1), _FLOATS[q.dtype], tokens, nq, k.shape[1], dim,
-          2 * inv_freq.numel(), positions.data_ptr(), int(positions.dtype == torch.int64), inv_freq.data_ptr(),
-          q_weight.data_ptr() if q_weight is not None else None, k_weight.data_ptr() if k_weight is not None else None,
-          _FLOATS[wtype or q.dtype], float(eps), int(bool(interleaved)))
+    if inplace:
+        qo, ko, qo0, qo1, ko0, ko1 = q, k, q0, q1, k0, k1
+    else:
+        qo, ko, qo0, qo1, ko0, ko1 = _empty_like(q), _empty_like(k), nq * dim, dim, nk * dim, dim
+    _call(device, _lib.lib().bh_op_qk_norm_rotary, qp, q0, q1, qo.data_ptr(), qo0, qo1, kp, k0, k1, ko.data_ptr(), ko0, ko1, _FLOATS[dtype], tokens,
+          nq, nk, dim, rotary, positions.data_ptr(), wide, inv_freq.data_ptr(), _ptr(q_weight), _ptr(k_weight), _FLOATS[wtype or dtype],
+          float(eps), bool(interleaved))
     if inplace:
         torch.autograd.graph.increment_version((q, k))
     return qo, ko
@@ -178,23 +190,23 @@ def kv_cache(pages, heads, page_size, dim, dtype=torch.bfloat16, device="cuda"):
 
 
 def _cache_tensors(k_cache, v_cache, k_scale, v_scale):
-    if not (k_cache.dim() == 4 and k_cache.dtype in _CACHES):
-        _fail(f"k_cache must be [pages, heads, page_size, dim], float16, bfloat16, int8 or float8_e4m3fn; " f"got {tuple(k_cache.shape)} {k_cache.dtype}")
-    if not (v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype):
+    """-> the cache's sizes and whether it is scaled."""
+    kind, shape = k_cache.dtype, k_cache.shape
+    if k_cache.dim() != 4 or kind not in _CACHES:
+        _fail(f"k_cache must be [pages, heads, page_size, dim], float16, bfloat16, int8 or float8_e4m3fn; got {tuple(shape)} {kind}")
+    if v_cache.shape != shape or v_cache.dtype != kind:
         _fail("v_cache must have k_cache's shape and type")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         _fail("k_cache and v_cache must be contiguous")
-    if k_cache.dtype in _SCALED:
-        for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
-            if not (s is not None and s.shape == k_cache.shape[:3] and s.dtype == torch.float32 and s.is_contiguous()):
-                _fail(f"an 8-bit cache needs {name}: contiguous float32 {tuple(k_cache.shape[:3])}")
-    else:
-        if not (k_scale is None and v_scale is None):
-            _fail(f"a cache of {k_cache.dtype} has no scales")
-
-
-def _ptr(t):
-    return t.data_ptr() if t is not None else None
+    scaled = kind in _SCALED
+    if scaled:
+        scales = shape[:3]
+        for s in (k_scale, v_scale):
+            if s is None or s.shape != scales or s.dtype != torch.float32 or not s.is_contiguous():
+                _fail(f"an 8-bit cache needs {'k_scale' if s is k_scale else 'v_scale'}: contiguous float32 {tuple(scales)}")
+    elif k_scale is not None or v_scale is not None:
+        _fail(f"a cache of {kind} has no scales")
+    return shape, scaled
 
 
 def kv_cache_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
@@ -204,36 +216,36 @@ def kv_cache_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
     exact quotient rounded to nearest even; float8_e4m3fn with the least power of two that keeps amax within 448.  A vector that holds an
     infinity or a NaN reads back as NaN.
     """
-    _cache_tensors(k_cache, v_cache, k_scale, v_scale)
-    pages, heads, page, dim = k_cache.shape
-    _rows("k", k, heads, dim)
-    _rows("v", v, heads, dim)
-    if not (v.shape == k.shape and v.dtype == k.dtype):
+    (pages, heads, page, dim), _ = _cache_tensors(k_cache, v_cache, k_scale, v_scale)
+    tokens, heads_k, dim_k, k0, k1, kp = _rows("k", k)
+    *same, v0, v1, vp = _rows("v", v)
+    if heads_k != heads or dim_k != dim:
+        _fail(f"k has shape {tuple(k.shape)}, the cache {heads} heads of {dim}")
+    if same != [tokens, heads, dim] or v.dtype != k.dtype:
         _fail("v must have k's shape and type")
-    if not (slots.shape == (k.shape[0],) and slots.dtype == torch.int64 and slots.is_contiguous()):
-        _fail(f"slots must be contiguous int64 [{k.shape[0]}]")
-    if k_cache.data_ptr() == v_cache.data_ptr() and k_cache.numel():
+    if slots.dtype != torch.int64 or slots.dim() != 1 or slots.shape[0] != tokens or not slots.is_contiguous():
+        _fail(f"slots must be contiguous int64 [{tokens}]")
+    kc, vc = k_cache.data_ptr(), v_cache.data_ptr()
+    if kc == vc and k_cache.numel():
         _fail("k_cache and v_cache are the same memory")
     device = _one_device("k v slots k_cache v_cache k_scale v_scale", k, v, slots, k_cache, v_cache, k_scale, v_scale)
-    _call(device, _lib.lib().bh_op_kv_write, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _FLOATS[k.dtype],
-          slots.data_ptr(), k.shape[0], heads, dim, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), _CACHES[k_cache.dtype],
-          pages, page)
+    _call(device, _lib.lib().bh_op_kv_write, kp, k0, k1, vp, v0, v1, _FLOATS[k.dtype], slots.data_ptr(), tokens, heads, dim, kc, vc, _ptr(k_scale),
+          _ptr(v_scale), _CACHES[k_cache.dtype], pages, page)
 
 
 def kv_cache_read(slots, k_cache, v_cache, k_scale=None, v_scale=None, dtype=torch.bfloat16):
     """The slots' keys and values (int64 [tokens]) as `dtype` -> (k, v) [tokens, heads, dim]; zeros for a slot outside the cache."""
-    _cache_tensors(k_cache, v_cache, k_scale, v_scale)
-    pages, heads, page, dim = k_cache.shape
-    if not (dtype in _FLOATS):
+    (pages, heads, page, dim), _ = _cache_tensors(k_cache, v_cache, k_scale, v_scale)
+    if dtype not in _FLOATS:
         _fail(f"dtype must be float16, bfloat16 or float32, got {dtype}")
-    if not (slots.dim() == 1 and slots.dtype == torch.int64 and slots.is_contiguous()):
+    if slots.dim() != 1 or slots.dtype != torch.int64 or not slots.is_contiguous():
         _fail("slots must be contiguous int64 [tokens]")
     device = _one_device("slots k_cache v_cache k_scale v_scale", slots, k_cache, v_cache, k_scale, v_scale)
-    k = slots.new_empty((slots.shape[0], heads, dim), dtype=dtype)
+    tokens = slots.shape[0]
+    k = slots.new_empty((tokens, heads, dim), dtype=dtype)
     v = torch.empty_like(k)
-    _call(device, _lib.lib().bh_op_kv_read, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _FLOATS[dtype],
-          slots.data_ptr(), slots.shape[0], heads, dim, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale),
-          _CACHES[k_cache.dtype], pages, page)
+    _call(device, _lib.lib().bh_op_kv_read, k.data_ptr(), heads * dim, dim, v.data_ptr(), heads * dim, dim, _FLOATS[dtype], slots.data_ptr(), tokens,
+          heads, dim, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), _CACHES[k_cache.dtype], pages, page)
     return k, v
 
 
@@ -248,28 +260,33 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, scale=None, k_sca
     float32: minus slope times the distance.  window w > 0: the last w tokens only.  lse [batch, n_q] float32: log of the sum of e^score.
     A sequence with nothing left gives zeros and -inf.
     """
-    _cache_tensors(k_cache, v_cache, k_scale, v_scale)
-    pages, heads, page, dim = k_cache.shape
-    _rows("q", q, dim=dim)
-    batch, nq, _ = q.shape
-    if not (q.dtype in (torch.float16, torch.bfloat16)):
-        _fail(f"q must be float16 or bfloat16, got {q.dtype}")
-    if not (k_cache.dtype == q.dtype or k_cache.dtype in _SCALED):
-        _fail(f"the cache must be {q.dtype}, int8 or float8_e4m3fn, got {k_cache.dtype}")
-    if not (block_table.dim() == 2 and block_table.shape[0] == batch and block_table.dtype == torch.int32 and (block_table.shape[1] <= 1 or block_table.stride(1) == 1)):
-        _fail(f"block_table must be int32 [{batch}, width] with dense rows")
-    if not (lengths.shape == (batch,) and lengths.dtype == torch.int32 and lengths.is_contiguous()):
+    (pages, heads, page, dim), scaled = _cache_tensors(k_cache, v_cache, k_scale, v_scale)
+    batch, nq, dim_q, q0, q1, qp = _rows("q", q)
+    dtype = q.dtype
+    if dim_q != dim:
+        _fail(f"q has shape {tuple(q.shape)}, the cache heads of {dim}")
+    if dtype == torch.float32:
+        _fail(f"q must be float16 or bfloat16, got {dtype}")
+    if not scaled and k_cache.dtype != dtype:
+        _fail(f"the cache must be {dtype}, int8 or float8_e4m3fn, got {k_cache.dtype}")
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.shape[0] != batch:
+        _fail(f"block_table must be int32 [{batch}, width]")
+    width, (t0, dense) = block_table.shape[1], block_table.stride()
+    if dense != 1 and width > 1:
+        _fail("block_table's rows must be dense")
+    if lengths.dtype != torch.int32 or lengths.dim() != 1 or lengths.shape[0] != batch or not lengths.is_contiguous():
         _fail(f"lengths must be contiguous int32 [{batch}]")
-    if alibi_slopes is not None:
-        if not (alibi_slopes.shape == (nq,) and alibi_slopes.dtype == torch.float32 and alibi_slopes.is_contiguous()):
-            _fail(f"alibi_slopes must be contiguous float32 [{nq}]")
+    if alibi_slopes is not None and (alibi_slopes.dim() != 1 or alibi_slopes.shape[0] != nq or alibi_slopes.dtype != torch.float32
+                                     or not alibi_slopes.is_contiguous()):
+        _fail(f"alibi_slopes must be contiguous float32 [{nq}]")
     if not 0 <= window < 1 << 31:
         _fail(f"window must be 0 or a count of tokens, got {window}")
     device = _one_device("q k_cache v_cache block_table lengths k_scale v_scale alibi_slopes", q, k_cache, v_cache, block_table, lengths, k_scale,
                          v_scale, alibi_slopes)
-    if q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8:
+    if qp % 16 or q0 % 8 or q1 % 8:
         q = q.contiguous()
-    lib, width = _lib.lib(), block_table.shape[1]
+        q0, q1, qp = nq * dim, dim, q.data_ptr()
+    lib = _lib.lib()
     need = lib.bh_op_paged_attention_workspace(batch, nq, heads, dim, page, width, int(window))
     if need < 0:
         _lib.check(need)
@@ -277,10 +294,9 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, scale=None, k_sca
     lse = q.new_empty((batch, nq), dtype=torch.float32) if return_lse else None
     # (made anew for each call: two calls at once, or two captured graphs, must not share one)
     work = lengths.new_empty(need, dtype=torch.uint8) if need else None
-    _call(device, lib.bh_op_paged_attention, q.data_ptr(), q.stride(0), q.stride(1), _FLOATS[q.dtype], k_cache.data_ptr(), v_cache.data_ptr(),
-          _ptr(k_scale), _ptr(v_scale), _CACHES[k_cache.dtype], pages, page, block_table.data_ptr(), block_table.stride(0), width,
-          lengths.data_ptr(), batch, nq, heads, dim, float(dim ** -0.5 if scale is None else scale), float(softcap), int(window),
-          _ptr(alibi_slopes), out.data_ptr(), _ptr(lse), _ptr(work), need)
+    _call(device, lib.bh_op_paged_attention, qp, q0, q1, _FLOATS[dtype], k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale),
+          _CACHES[k_cache.dtype], pages, page, block_table.data_ptr(), t0, width, lengths.data_ptr(), batch, nq, heads, dim,
+          float(dim ** -0.5 if scale is None else scale), float(softcap), int(window), _ptr(alibi_slopes), out.data_ptr(), _ptr(lse), _ptr(work), need)
     return (out, lse) if return_lse else out
 
 
@@ -292,20 +308,22 @@ def token_logprobs(logits, targets, top=0):
     A negative target's log probability is 0 (padding), one beyond the vocabulary NaN.  -inf logits carry no probability; a row of nothing
     else has log probabilities -inf and entropy 0; a row with a NaN or +inf has NaN.  top is at most 64.
     """
-    if not (logits.dim() == 2 and logits.dtype in _FLOATS):
+    if logits.dim() != 2 or logits.dtype not in _FLOATS:
         _fail(f"logits must be [rows, vocab], float16, bfloat16 or float32; got {tuple(logits.shape)} {logits.dtype}")
-    rows, vocab = logits.shape
-    if not (vocab >= 1 and (vocab == 1 or logits.stride(1) == 1)):
+    (rows, vocab), (by_row, dense) = logits.shape, logits.stride()
+    if vocab < 1 or (dense != 1 and vocab > 1):
         _fail("logits' rows must be dense and not empty")
-    if not (targets.dtype == torch.int64 and targets.dim() in (1, 2) and targets.shape[0] == rows and targets.is_contiguous()):
+    given = targets.dim()
+    if targets.dtype != torch.int64 or not 1 <= given <= 2 or targets.shape[0] != rows or not targets.is_contiguous():
         _fail(f"targets must be contiguous int64 [{rows}] or [{rows}, given]")
+    given = 1 if given == 1 else targets.shape[1]
     if not 0 <= top <= vocab:
         _fail(f"top {top} of {vocab} tokens")
     device = _one_device("logits targets", logits, targets)
-    if rows > 1 and logits.stride(0) < vocab:
-        logits = logits.contiguous()
-    lib, top = _lib.lib(), int(top)
-    need = lib.bh_op_token_logprobs_workspace(rows, vocab, _FLOATS[logits.dtype], top)
+    if rows > 1 and by_row < vocab:
+        logits, by_row = logits.contiguous(), vocab
+    lib, code, top = _lib.lib(), _FLOATS[logits.dtype], int(top)
+    need = lib.bh_op_token_logprobs_workspace(rows, vocab, code, top)
     if need < 0:
         _lib.check(need)
     logprobs = logits.new_empty(targets.shape, dtype=torch.float32)
@@ -313,7 +331,6 @@ def token_logprobs(logits, targets, top=0):
     top_logprobs = logits.new_empty((rows, top), dtype=torch.float32)
     top_ids = targets.new_empty((rows, top))
     work = targets.new_empty(need, dtype=torch.uint8) if need else None
-    _call(device, lib.bh_op_token_logprobs, logits.data_ptr(), logits.stride(0), _FLOATS[logits.dtype], rows, vocab, targets.data_ptr(),
-          1 if targets.dim() == 1 else targets.shape[1], top, logprobs.data_ptr(), entropy.data_ptr(), top_logprobs.data_ptr(),
-          top_ids.data_ptr(), _ptr(work), need)
+    _call(device, lib.bh_op_token_logprobs, logits.data_ptr(), by_row, code, rows, vocab, targets.data_ptr(), given, top, logprobs.data_ptr(),
+          entropy.data_ptr(), top_logprobs.data_ptr(), top_ids.data_ptr(), _ptr(work), need)
     return TokenLogprobs(logprobs, entropy, top_logprobs, top_ids)

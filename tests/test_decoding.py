@@ -29,7 +29,7 @@ _QKV = torch.zeros(3, 8, 64, dtype=torch.bfloat16)
 @pytest.mark.parametrize("change, match", [
     (dict(q=torch.zeros(3, 4, dtype=torch.bfloat16)), r"q must be \[tokens, heads, dim\]"),
     (dict(q=torch.zeros(3, 4, 64, dtype=torch.float64)), "float16, bfloat16 or float32"),
-    (dict(k=torch.zeros(3, 2, 32, dtype=torch.bfloat16)), "k has shape"),
+    (dict(k=torch.zeros(3, 2, 32, dtype=torch.bfloat16)), "k must be"),
     (dict(k=torch.zeros(2, 2, 64, dtype=torch.bfloat16)), "k must be"),
     (dict(k=torch.zeros(3, 2, 64, dtype=torch.float16)), "k must be"),
     (dict(positions=torch.zeros(3)), "positions"),
