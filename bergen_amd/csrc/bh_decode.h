@@ -1,22 +1,11 @@
 // bh_decode.h — what the operators of a decoding step share (decode_ops.hip, paged_attention.hip, token_logprobs.hip): element
-// types, 16-byte loads as fp32, group reductions.
+// types, group reductions.
 #pragma once
 #include "bh_device.h"
 #include "bh_host.h"
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-
-struct BhF16 {
-    typedef _Float16 elem;
-};
-struct BhBf16 {
-    typedef __bf16 elem;
-};
-struct BhF32 {
-    typedef float elem;
-};
 
 inline size_t bh_dtype_size(int32_t dtype) {
     return dtype == BH_F32 ? 4 : dtype == BH_F16 || dtype == BH_BF16 ? 2 : dtype == BH_I8 || dtype == BH_E4M3 ? 1 : 0;
@@ -25,41 +14,14 @@ inline bool bh_is_float(int32_t dtype) { return dtype == BH_F16 || dtype == BH_B
 
 inline bool bh_aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-// 8 consecutive elements at p (16-byte aligned) as fp32 / from fp32, rounded to nearest even.
-template <typename E>
-__device__ __forceinline__ void bh_load8(const E* p, float (&x)[8]) {
-    typedef E vec __attribute__((ext_vector_type(8)));
-    const vec v = *reinterpret_cast<const vec*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
-}
-template <>
-__device__ __forceinline__ void bh_load8<float>(const float* p, float (&x)[8]) {
+// 8 consecutive numbers at p (16-byte aligned).
+__device__ __forceinline__ void bh_load8(const float* p, float (&x)[8]) {
     const floatx4 a = *reinterpret_cast<const floatx4*>(p), b = *reinterpret_cast<const floatx4*>(p + 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         x[i] = a[i];
         x[4 + i] = b[i];
     }
-}
-template <typename E>
-__device__ __forceinline__ void bh_store8(E* p, const float (&x)[8]) {
-    typedef E vec __attribute__((ext_vector_type(8)));
-    vec v;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (E)x[i];
-    *reinterpret_cast<vec*>(p) = v;
-}
-template <>
-__device__ __forceinline__ void bh_store8<float>(float* p, const float (&x)[8]) {
-    floatx4 a, b;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        a[i] = x[i];
-        b[i] = x[4 + i];
-    }
-    *reinterpret_cast<floatx4*>(p) = a;
-    *reinterpret_cast<floatx4*>(p + 4) = b;
 }
 
 // Reductions over aligned groups of `size` lanes (a power of two).

@@ -1,5 +1,5 @@
 """Plain implementations, in 64 bits, of the decoding operators (bergen_amd/decoding.py), with bounds on how far a kernel that
-computes in 32 bits and rounds once may be from them.  Checkers of the tests only."""
+computes in 32 bits and rounds once may be from them.  Used by the tests only."""
 import math
 
 import torch

@@ -1,5 +1,5 @@
 """CPU: the decoding operators' checks of arguments (bergen_amd/decoding.py and the C entry points), which come before anything
-touches a device, and the checker's own formulas against differences it does not share."""
+touches a device, and the reference's own formulas against torch's."""
 import ctypes
 import math
 
@@ -176,8 +176,8 @@ def test_rotary_frequencies():
     _refused("even", bergen_amd.rotary_frequencies, 7, device="cpu")
 
 
-def test_the_checker_against_torch():
-    """The 64-bit checkers agree with torch's own functions where torch has one."""
+def test_the_reference_against_torch():
+    """The 64-bit formulas agree with torch's own functions where torch has one."""
     g = torch.Generator().manual_seed(0)
     x = torch.randn(5, 301, generator=g)
     r = ref.logprobs(x, torch.arange(5), 7)
