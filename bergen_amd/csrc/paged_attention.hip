@@ -7,7 +7,7 @@
 // head alone makes 1 flop per byte, a group of 8 makes 8; on the vector units 8 would already take all their cycles, so both products run
 // on the matrix cores, 16 heads wide whether there are 16 or 1 (the matrix pipe is busy 5 % of the time for 4 heads a group in bf16).
 // Measured: 64 sequences of 90..8191 tokens, 8 key heads of 128, bf16: 186 us = 5.8 TB/s (the loads alone: 189 us); 3 of 100001..131072 tokens, e4m3: 145 us
-// = 5.0 TB/s (the loads alone: 135 us); 37 of 1..6000, window 4096, 12 heads of 64 without groups, int8: 42 us = 3.8 TB/s (the loads alone 31 us: the
+// = 5.0 TB/s (the loads alone: 135 us); 37 of 1..6000, window 4096, 12 heads of 64 without groups, int8: 44 us = 3.7 TB/s (the loads alone 31 us: the
 // vector instructions of a tile are the same for 1 head as for 16).
 //
 // A wave takes 32 tokens of one key head at a time and needs no LDS for them:
@@ -337,12 +337,23 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : DP == 64 ? 4 : EXA
             }
 
             // ---- softmax: the lane's 8 tokens of head n
-            if (a.softcap > 0.f) {
+            auto capped = [&](float x) {
+                const float e2 = __builtin_amdgcn_exp2f(fminf(x * cap_unit, 64.f));  // e^(2 s / c)
+                return x == x ? cap * (e2 - 1.f) * __builtin_amdgcn_rcpf(e2 + 1.f) : x;
+            };
+            if (a.softcap > 128.f) {
+                // e2 - 1 keeps 2^-23 of 1, which times a large cap is more than a score may be off by: below c / 4 tanh's series, whose first
+                // term left out is 9e-9 of the score.  (Being there it costs low caps 2 us of 44, in a loop of its own as well; both forms with a
+                // choice for each score cost 5)
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
-                    const float e2 = __builtin_amdgcn_exp2f(fminf(x[r] * cap_unit, 64.f));  // e^(2 s / c)
-                    x[r] = x[r] == x[r] ? cap * (e2 - 1.f) * __builtin_amdgcn_rcpf(e2 + 1.f) : x[r];
+                    const float z = x[r] * cap_unit * (0.5f * LN2), z2 = z * z;
+                    const float series = x[r] + x[r] * (z2 * (-1.f / 3 + z2 * (2.f / 15 + z2 * (-17.f / 315 + z2 * (62.f / 2835)))));
+                    x[r] = fabsf(z) < 0.25f ? series : capped(x[r]);
                 }
+            } else if (a.softcap > 0.f) {
+#pragma unroll
+                for (int r = 0; r < 8; ++r) x[r] = capped(x[r]);
             }
             if (a.slopes) {
                 const float by = DP > 64 ? sh_stats[wave][0][n] : slope;

@@ -287,6 +287,23 @@ def test_attention_of_long_sequences(cache):
     assert torch.equal(one[0], check_attention(q[3:4], c, table[3:4], lengths[3:4])[0])  # the same call, the same bits
 
 
+@pytest.mark.parametrize("softcap", [127.0, 129.0, 1e4, 1e7, 1e30])
+@pytest.mark.parametrize("cache, dim", [(BF, 64), (I8, 128), (E4, 256)])
+def test_attention_with_a_high_cap(cache, dim, softcap):
+    """A cap far above the scores leaves them as they are, to their own roundings: tanh adds less than 14 x 2^-24 of a score, and the plain bound holds
+    dim + 16 of those.  Below 128 the cap's own 8 x 2^-24 is allowed for."""
+    g = gen(int(softcap % 1000) + dim)
+    lengths = [1, 40, 333]
+    c = made_cache(g, 40, 2, 16, dim, cache)
+    table = table_for(g, lengths, 16, 40)
+    q, n = 6 * randn(g, 3, 4, dim, dtype=BF), torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    got, lse = bergen_amd.paged_attention(q, c.k_cache, c.v_cache, table, n, k_scale=c.k_scale, v_scale=c.v_scale, softcap=softcap, return_lse=True)
+    want, cap_bound, wlse, cap_lbound = ref.attention(q, c.k_cache, c.v_cache, table, n, None, c.k_scale, c.v_scale, softcap)
+    _, bound, _, lbound = ref.attention(q, c.k_cache, c.v_cache, table, n, None, c.k_scale, c.v_scale)
+    ref.assert_within(lse, wlse, cap_lbound if softcap < 128 else 2 * lbound, "lse")
+    ref.assert_within(got, want, cap_bound if softcap < 128 else 2 * bound, "out")
+
+
 @pytest.mark.parametrize("cache", [BF, I8])
 def test_attention_without_some_pages(cache):
     """Table entries outside the cache: their tokens are left out; where all are, zeros and -inf.  Lengths outside the table's width."""
