@@ -284,7 +284,7 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, scale=None, k_sca
     device = _one_device("q k_cache v_cache block_table lengths k_scale v_scale alibi_slopes", q, k_cache, v_cache, block_table, lengths, k_scale,
                          v_scale, alibi_slopes)
     if qp % 16 or q0 % 8 or q1 % 8:
-        q = q.contiguous()
+        q = q.clone(memory_format=torch.contiguous_format)  # (contiguous() would hand back a dense one that starts off a border)
         q0, q1, qp = nq * dim, dim, q.data_ptr()
     lib = _lib.lib()
     need = lib.bh_op_paged_attention_workspace(batch, nq, heads, dim, page, width, int(window))

@@ -304,6 +304,20 @@ def test_attention_with_a_high_cap(cache, dim, softcap):
     ref.assert_within(got, want, cap_bound if softcap < 128 else 2 * bound, "out")
 
 
+def test_attention_of_queries_off_a_border():
+    """Dense queries that start 2 bytes behind a 16-byte border, and slices of rows of odd length, give what aligned ones do."""
+    g = gen(14)
+    c, n = made_cache(g, 12, 2, 16, 64, BF), torch.tensor([20, 60], dtype=torch.int32, device="cuda")
+    table = table_for(g, [20, 60], 16, 12, 0)
+    q = randn(g, 2, 4, 64, dtype=BF)
+    want = bergen_amd.paged_attention(q, c.k_cache, c.v_cache, table, n)
+    off = torch.empty(513, dtype=BF, device="cuda")[1:].view(2, 4, 64).copy_(q)
+    odd = torch.empty(2, 4, 65, dtype=BF, device="cuda")[..., 1:].copy_(q)
+    assert off.is_contiguous() and off.data_ptr() % 16 == 2
+    for x in (off, odd):
+        assert torch.equal(bergen_amd.paged_attention(x, c.k_cache, c.v_cache, table, n), want)
+
+
 @pytest.mark.parametrize("cache", [BF, I8])
 def test_attention_without_some_pages(cache):
     """Table entries outside the cache: their tokens are left out; where all are, zeros and -inf.  Lengths outside the table's width."""
