@@ -231,6 +231,7 @@ def kv_cache_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
     device = _one_device("k v slots k_cache v_cache k_scale v_scale", k, v, slots, k_cache, v_cache, k_scale, v_scale)
     _call(device, _lib.lib().bh_op_kv_write, kp, k0, k1, vp, v0, v1, _FLOATS[k.dtype], slots.data_ptr(), tokens, heads, dim, kc, vc, _ptr(k_scale),
           _ptr(v_scale), _CACHES[k_cache.dtype], pages, page)
+    torch.autograd.graph.increment_version([t for t in (k_cache, v_cache, k_scale, v_scale) if t is not None])
 
 
 def kv_cache_read(slots, k_cache, v_cache, k_scale=None, v_scale=None, dtype=torch.bfloat16):

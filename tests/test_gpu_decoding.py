@@ -141,6 +141,19 @@ def test_cache(cache, dtype, tokens, heads, dim, page):
         assert torch.equal(a.transpose(1, 2)[~touched], b.transpose(1, 2)[~touched])
 
 
+@pytest.mark.parametrize("cache", [BF, E4])
+def test_a_write_is_told_to_autograd(cache):
+    """A backward pass that needs what the cache held before a write is refused, as after torch's own writes in place."""
+    c = bergen_amd.kv_cache(2, 1, 8, 16, cache)
+    held = c.v_scale if cache is E4 else c.v_cache
+    w = torch.ones_like(held, requires_grad=True)
+    y = (w * held).sum()
+    with torch.no_grad():
+        bergen_amd.kv_cache_write(torch.ones(1, 1, 16, device="cuda"), torch.ones(1, 1, 16, device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda"), *c)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
 @pytest.mark.parametrize("dim", [64, 50])
 @pytest.mark.parametrize("cache", [I8, E4])
 def test_quantising_borders(cache, dim):
