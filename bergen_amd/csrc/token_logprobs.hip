@@ -179,6 +179,8 @@ template <typename E, bool TOP>
 __global__ void __launch_bounds__(THREADS, 4) bh_token_logprobs_kernel(LogprobArgs a) {
     constexpr int MANY = 8, N = Vec<E>::N, U = 4;  // elements of a vector, vectors of a lane's step
     typedef float Step __attribute__((ext_vector_type(U * N)));
+    // the mode register's IEEE bit off: with it a maximum of a number and a signalling NaN is NaN, and the number would be lost to the alternatives
+    __builtin_amdgcn_s_setreg(1 /* MODE */ | 9 << 6 /* bit 9 */ | 0 << 11 /* one bit */, 0);
     __shared__ Shared<TOP ? WAVES * 64 : 1> sh;
     __shared__ u64 lists[TOP ? WAVES * 64 : 1];  // the waves' own
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

@@ -493,6 +493,21 @@ def test_logprobs_rows_and_ties(dtype):
     assert abs(float(r.entropy[0]) - math.log(n)) < 1e-5 and torch.isnan(r.logprobs[12]).all()
 
 
+@pytest.mark.parametrize("dtype, bits, signalling", [(BF, torch.int16, 0x7f81), (F32, torch.int32, 0x7f800001), (HF, torch.int16, 0x7c01)])
+def test_logprobs_next_to_a_signalling_nan(dtype, bits, signalling):
+    """It spoils its row's probabilities, as any NaN does, and hides no alternative: the largest logit beside it, in each place of a 16-byte vector."""
+    g = gen(8)
+    x, t = randn(g, 300, 50000, dtype=dtype), torch.zeros(300, dtype=torch.int64, device="cuda")
+    rows, at = torch.arange(16, device="cuda"), 40000 + torch.arange(16, device="cuda")
+    x[rows, at] = 50.0
+    x.view(bits)[rows, at ^ 1] = signalling
+    r = bergen_amd.token_logprobs(x, t, top=4)
+    assert torch.equal(r.top_ids[:16, 0], at)
+    assert torch.isnan(r.logprobs[:16]).all() and torch.isnan(r.top_logprobs[:16]).all() and torch.isfinite(r.logprobs[16:]).all()
+    whole = x.float().nan_to_num(nan=-math.inf)  # (every alternative of these rows is a number)
+    assert torch.equal(r.top_ids, torch.sort(whole, dim=-1, descending=True, stable=True).indices[:, :4])
+
+
 @pytest.mark.parametrize("dtype", [BF, HF, F32])
 def test_logprobs_of_a_types_limits(dtype):
     """The type's lowest value as a mask, in a whole row too (which is then uniform), its largest, its smallest, and a row of NaN alone."""
