@@ -29,12 +29,21 @@ struct RotaryArgs {
     bool pos64, w32, interleaved;
 };
 
-// cos and sin of pos * f, f in radians per position: the angle is formed and reduced to a fraction of a turn in 64 bits (fp32
-// would lose 2^-24 of an angle that reaches 1e6 and more), its sine and cosine are taken in 32.
+// cos and sin of pos * f, f in radians per position.  The angle is formed, reduced to a fraction of a turn and to |x| <= pi / 4 in 64 bits, and so are
+// the two Taylor series (the terms left out are below 2^-37 there): the results are the nearest fp32 numbers but for ties that close.  (A fraction
+// narrowed to fp32 before its sine moves the angle by up to 2^-23.4, which doubled the outputs that round the other way than the exact ones in bf16.)
 __device__ __forceinline__ void angle_of(double pos, double f, float& c, float& s) {
     double t = pos * f * 0.15915494309189533577;  // 1 / (2 pi)
     t -= rint(t);
-    sincospif(2.0f * (float)t, &s, &c);
+    const double quarters = rint(4.0 * t), x = (t - 0.25 * quarters) * 6.283185307179586477, z = x * x;
+    const double sn = x + x * z * (-1.0 / 6 + z * (1.0 / 120 + z * (-1.0 / 5040 + z * (1.0 / 362880 + z * (-1.0 / 39916800)))));
+    const double cs = 1.0 + z * (-0.5 + z * (1.0 / 24 + z * (-1.0 / 720 + z * (1.0 / 40320 + z * (-1.0 / 3628800 + z * (1.0 / 479001600))))));
+    const float a = (float)cs, b = (float)sn;
+    const bool odd = fabs(quarters) == 1.0;                           // (a NaN: no quarter at all, and both series are NaN)
+    const bool half = fabs(quarters) == 2.0, third = quarters < 0.0;  // -1 quarter: three of them
+    const float u = odd ? b : a, v = odd ? a : b;
+    c = half || (odd && !third) ? -u : u;
+    s = half || (odd && third) ? -v : v;
 }
 
 __device__ __forceinline__ double position(const RotaryArgs& a, long long t) {

@@ -90,6 +90,21 @@ def test_rotary_far_positions_and_values():
     assert torch.isnan(out[2, 1]).all()
 
 
+@pytest.mark.parametrize("dim, interleaved", [(128, False), (128, True), (100, False), (30, True)])
+def test_rotary_sines(dim, interleaved):
+    """Pairs (1, 0) come out as the cosine and sine themselves, with no rounding but their own: half a step of fp32, the angle's three roundings in 64 bits (the
+    test's own product is one more) and the series' 2^-36."""
+    pos = torch.cat([torch.arange(2000), torch.tensor([131071, 1 << 20, (1 << 31) - 1])]).cuda()
+    f = torch.cat([bergen_amd.rotary_frequencies(dim)[: dim // 2 - 5], torch.tensor([math.pi / 4, math.pi / 2, math.pi, -math.pi / 2, -0.1], device="cuda").double()])
+    a, b = (slice(0, dim, 2), slice(1, dim, 2)) if interleaved else (slice(0, dim // 2), slice(dim // 2, dim))
+    q = torch.zeros(len(pos), 1, dim, device="cuda")
+    q[..., a] = 1
+    out, _ = bergen_amd.qk_norm_rotary(q, q, pos, f, interleaved=interleaved)
+    angle = pos.cpu().double()[:, None] * f.cpu()
+    for got, want in ((out[:, 0, a], angle.cos()), (out[:, 0, b], angle.sin())):
+        ref.assert_within(got, want, 2.0 ** -24 * want.abs() + 4 * 2.0 ** -53 * angle.abs() + 2.0 ** -36, "sine")
+
+
 def test_rotary_of_nothing():
     q, k = torch.zeros(0, 4, 64, dtype=BF, device="cuda"), torch.zeros(0, 2, 64, dtype=BF, device="cuda")
     a, b = bergen_amd.qk_norm_rotary(q, k, torch.zeros(0, dtype=torch.int64, device="cuda"), bergen_amd.rotary_frequencies(64))
