@@ -17,7 +17,9 @@
 namespace {
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
-constexpr float FAR = 1e37f;
+// Beyond this magnitude of the running maximum m the exponents are taken from m itself.  Below it m log2(e) < 2^20.53, so that what its rounding leaves is at
+// most 2^-4 (2^off2 of 0.957 .. 1.045); it grows with m, and from about 3e9 on 2^off2 is infinity or zero.
+constexpr float FAR = 0x1p20f;
 constexpr int MAX_TOP = 64, WAVES = 4, THREADS = 64 * WAVES;
 
 struct LogprobArgs {
@@ -194,7 +196,7 @@ __global__ void __launch_bounds__(THREADS, 4) bh_token_logprobs_kernel(LogprobAr
     Seen s{-INFINITY, 0.f, 0.f, false};  // m: the wave's; rest, first: the lane's
     float m2 = 0.f;                      // m log2(e), rounded (0 while there is nothing but -inf): what the exponents are taken from, and
     float off2 = 0.f;                    // what the rounding left of it: 2^off2 is the maximum's own weight, put right at the end
-    bool huge = false;                   // m log2(e) is beyond fp32 (a row of nothing but the type's lowest value): exponents from m itself
+    bool huge = false;                   // m is beyond FAR (masked tokens of -1e10, the type's lowest value): exponents from m itself, m2 and off2 are 0
     u64 best = 0, bar = 0;               // the lane's key of the wave's list; the k-th key: what is not above it cannot be among the k
     float bar_x = __uint_as_float(0x7fc00000u);  // its value; a NaN lets everything through
 
@@ -293,8 +295,13 @@ __global__ void __launch_bounds__(THREADS, 4) bh_token_logprobs_kernel(LogprobAr
         }
         if (__any(step_most > s.m)) {  // a new maximum: a few times in a row
             const float top_x = wave_max(step_most);
+            const bool far = fabsf(top_x) > FAR;
+            float top2 = far ? 0.f : top_x * LOG2E;
+            asm("" : "+v"(top2));  // the ROUNDED product in every use: fused into the difference below it moved the sums by up to 2^off2 (5e-3 at 1e5)
+            const float top_off = far ? 0.f : fmaf(top_x, LOG2E, -top2);
             if (s.m > -INFINITY && top_x < INFINITY) {
-                const float by = huge || fabsf(top_x) > FAR ? (s.m - top_x) * LOG2E : m2 - __fmul_rn(top_x, LOG2E), f = __builtin_amdgcn_exp2f(by);
+                // from the old base to the new one; each is its maximum's exponent less its off2
+                const float by = huge || far ? (s.m - top_x) * LOG2E + (top_off - off2) : m2 - top2, f = __builtin_amdgcn_exp2f(by);
                 if (lane == 0) {  // the old maximum is one of many now
                     const float own = __builtin_amdgcn_exp2f(off2);
                     s.rest += own;
@@ -304,9 +311,9 @@ __global__ void __launch_bounds__(THREADS, 4) bh_token_logprobs_kernel(LogprobAr
                 s.rest *= f;
             }
             s.m = top_x;
-            huge = fabsf(top_x) > FAR;
-            m2 = huge ? 0.f : __fmul_rn(top_x, LOG2E);
-            off2 = huge ? 0.f : fmaf(top_x, LOG2E, -m2);
+            huge = far;
+            m2 = top2;
+            off2 = top_off;
             // its own 1 is left out: one element that equals it, of one lane
             bool mine = lane == __ffsll((unsigned long long)__ballot(step_most == top_x)) - 1;
 #pragma unroll

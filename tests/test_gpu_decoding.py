@@ -546,6 +546,46 @@ def test_logprobs_of_a_types_limits(dtype):
     check_logprobs(parts, torch.tensor([69000], device="cuda"), 3)
 
 
+def masked_rows(dtype, mask, n):
+    """Rows of n logits beside, below or above the finite value `mask`: it alone, two allowed tokens in many places, one maximum, steps of one unit up and down."""
+    base = torch.tensor(mask, dtype=dtype).double()
+    unit = 2.0 ** (math.floor(math.log2(abs(float(base)))) - {F32: 23, BF: 7}[dtype])
+    rows = [torch.full((n,), float(base), dtype=torch.float64)]
+    for yes, no in ((3, 4), (n // 2, n - 3), (n - 1, 70), (0, n // 3)):
+        x = torch.full((n,), float(base), dtype=torch.float64)
+        x[yes], x[no] = 1.5, 0.25
+        rows.append(x)
+    one = torch.full((n,), -math.inf, dtype=torch.float64)
+    one[n // 2 + 5] = base
+    steps = torch.arange(n, dtype=torch.float64) % 97
+    up = base + unit * torch.div(torch.arange(n), n // 60, rounding_mode="floor")  # a new maximum in every part of the row
+    rows += [one, base + unit * steps, base - unit * steps, up, up.flip(0), torch.where(steps == 5, -base, base)]
+    return torch.stack(rows).to(dtype).cuda()
+
+
+@pytest.mark.parametrize("mask", [-1e4, -1e5, -1048573.0, -1.0486e6, -1e7, -1e9, -1e10, -1e11, -1e12, -1e20, -1e30])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_logprobs_of_finite_masks(dtype, mask):
+    """Every magnitude of the maximum, on both sides of zero, in a row of several parts and in rows that one workgroup walks in several steps."""
+    for sign in (1, -1):
+        x = masked_rows(dtype, sign * mask, 20011)
+        t = torch.tensor([3, 10005, 20010, 0, 777], device="cuda").expand(x.shape[0], 5).contiguous()
+        for top in (0, 5):
+            r = check_logprobs(x, t, top)
+            assert torch.isfinite(r.entropy).all()
+        many = bergen_amd.token_logprobs(x.repeat(100, 1), t.repeat(100, 1), top=5)     # 1100 rows: each in one part
+        want = ref.logprobs(x, t, 5)
+        for i in (0, 1, 99):
+            part = slice(i * len(x), (i + 1) * len(x))
+            ref.assert_within(many.logprobs[part], *want["logprobs"], "logprobs")
+            ref.assert_within(many.entropy[part], *want["entropy"], "entropy")
+            ref.assert_within(many.top_logprobs[part], *want["top_logprobs"], "top_logprobs")
+            assert torch.equal(many.top_ids[part].cpu(), want["top_ids"])
+    parts = torch.full((1, 70000), mask, device="cuda", dtype=dtype)                    # several parts, allowed tokens in the last one only
+    parts[0, 69990], parts[0, 69999] = 2.0, 1.0
+    check_logprobs(parts, torch.tensor([[69990, 69999]], device="cuda"), 3)
+
+
 def test_entropy_of_a_nearly_certain_row():
     """p = 1 - 1e-9: the entropy is kept, not rounded to 0."""
     x = torch.full((2, 1000), -math.inf, device="cuda")
