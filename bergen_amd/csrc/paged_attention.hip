@@ -193,7 +193,10 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : DP == 64 ? 4 : EXA
         }
     }
     const float slope = a.slopes && head_live ? a.slopes[hq0 + n] * LOG2E : 0.f;
-    if (DP > 64 && g == 0) sh_stats[wave][0][n] = slope;  // (kept there until the wave's own m comes; heads of 64 keep it in a register)
+    if (DP > 64) {
+        if (g == 0) sh_stats[wave][0][n] = slope;  // (kept there until the wave's own m comes; heads of 64 keep it in a register)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the other lanes of the wave read it: not before the store
+    }
     const float cap = a.softcap * LOG2E, cap_unit = a.softcap > 0.f ? 2.f / a.softcap : 0.f;
 
     float m, total;  // of head n: the same m in its 4 lanes; each lane's own sum, times 2^HOLD

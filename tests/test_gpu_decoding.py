@@ -332,6 +332,19 @@ def test_attention_with_a_high_cap(cache, dim, softcap):
     ref.assert_within(got, want, cap_bound if softcap < 128 else 2 * bound, "out")
 
 
+@pytest.mark.parametrize("cache", [BF, I8, E4])
+@pytest.mark.parametrize("dim", [64, 80, 128, 256])
+def test_attention_where_the_distance_decides(dim, cache):
+    """Keys of zeros: the weights are the slopes' alone, another one in each of 20 heads of a group (16 and 4 of them in a workgroup)."""
+    g = gen(dim)
+    lengths = [1, 33, 200, 1500]
+    pages = sum(-(-n // 16) for n in lengths)
+    c = made_cache(g, pages, 2, 16, dim, cache)
+    c.k_cache.view(torch.int8 if cache != BF else torch.int16).zero_()
+    slopes = torch.exp2(-12 * torch.rand(40, generator=g, device="cuda"))
+    check_attention(randn(g, 4, 40, dim, dtype=BF), c, table_for(g, lengths, 16, pages, 0), lengths, slopes=slopes)
+
+
 def test_attention_of_queries_off_a_border():
     """Dense queries that start 2 bytes behind a 16-byte border, and slices of rows of odd length, give what aligned ones do."""
     g = gen(14)
