@@ -212,11 +212,12 @@ def _cache_tensors(k_cache, v_cache, k_scale, v_scale):
 def kv_cache_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
     """Rows k, v [tokens, heads, dim] (float16, bfloat16 or float32) into their slots (int64 [tokens]; page * page_size + offset) of the cache.
 
-    A slot outside the cache, -1 for padding, is skipped; the slots of one call must differ.  8-bit caches: int8 with scale = amax / 127 and the
+    A slot outside the cache, -1 for padding, is skipped; the slots of one call must differ, and k and v must not be vectors of the cache that it
+    writes.  8-bit caches: int8 with scale = amax / 127 and the
     exact quotient rounded to nearest even; float8_e4m3fn with the least power of two that keeps amax within 448.  A vector that holds an
     infinity or a NaN reads back as NaN.
     """
-    (pages, heads, page, dim), _ = _cache_tensors(k_cache, v_cache, k_scale, v_scale)
+    (pages, heads, page, dim), scaled = _cache_tensors(k_cache, v_cache, k_scale, v_scale)
     tokens, heads_k, dim_k, k0, k1, kp = _rows("k", k)
     *same, v0, v1, vp = _rows("v", v)
     if heads_k != heads or dim_k != dim:
@@ -226,8 +227,17 @@ def kv_cache_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
     if slots.dtype != torch.int64 or slots.dim() != 1 or slots.shape[0] != tokens or not slots.is_contiguous():
         _fail(f"slots must be contiguous int64 [{tokens}]")
     kc, vc = k_cache.data_ptr(), v_cache.data_ptr()
-    if kc == vc and k_cache.numel():
-        _fail("k_cache and v_cache are the same memory")
+    size = k_cache.numel() * k_cache.element_size()
+    if kc < vc + size and vc < kc + size:
+        _fail("k_cache and v_cache are the same memory, or share some")
+    if scaled:
+        ks, vs, size_s = k_scale.data_ptr(), v_scale.data_ptr(), 4 * k_scale.numel()
+        if ks < vs + size_s and vs < ks + size_s:
+            _fail("k_scale and v_scale are the same memory, or share some")
+        for codes in (kc, vc):
+            for scales in (ks, vs):
+                if codes < scales + size_s and scales < codes + size:
+                    _fail("the cache's codes and its scales share memory")
     device = _one_device("k v slots k_cache v_cache k_scale v_scale", k, v, slots, k_cache, v_cache, k_scale, v_scale)
     _call(device, _lib.lib().bh_op_kv_write, kp, k0, k1, vp, v0, v1, _FLOATS[k.dtype], slots.data_ptr(), tokens, heads, dim, kc, vc, _ptr(k_scale),
           _ptr(v_scale), _CACHES[k_cache.dtype], pages, page)

@@ -79,6 +79,26 @@ def test_cache_refusals():
     _refused("a cache holds", bergen_amd.kv_cache, 1, 1, 16, 32, torch.float32, device="cpu")
 
 
+def test_cache_memory_that_is_shared():
+    """Keys and values are written at once: caches, scales, or codes and scales that meet anywhere are refused; those that lie side by side are not."""
+    k, slots = torch.zeros(5, 3, 32), torch.zeros(5, dtype=torch.int64)
+    a = _cache_args()
+    both = torch.zeros(3, 3, 16, 32, dtype=torch.int8)
+    scales = torch.zeros(3, 3, 16)
+    raw = torch.zeros(4 * 3072, dtype=torch.int8)
+    for change, match in [(dict(v_scale=a["k_scale"]), "k_scale and v_scale are the same memory"), (dict(k_cache=both[:2], v_cache=both[1:]), "share some"),
+                          (dict(k_cache=both[1:], v_cache=both[:2]), "share some"), (dict(k_scale=scales[:2], v_scale=scales[1:]), "share some"),
+                          (dict(k_cache=raw[:3072].view(2, 3, 16, 32), k_scale=raw[3008:3392].view(torch.float32).view(2, 3, 16)), "codes and its scales"),
+                          (dict(v_cache=raw[3072:6144].view(2, 3, 16, 32), k_scale=raw[2816:3200].view(torch.float32).view(2, 3, 16)), "codes and its scales"),
+                          (dict(k_cache=raw[:3072].view(2, 3, 16, 32), v_cache=raw[3072:6144].view(2, 3, 16, 32), k_scale=raw[6144:6528].view(torch.float32).view(2, 3, 16),
+                                v_scale=raw[6528:6912].view(torch.float32).view(2, 3, 16)), "must be on the GPU")]:
+        _refused(match, bergen_amd.kv_cache_write, k, k, slots, **{**a, **change})
+    half = torch.zeros(3, 3, 16, 32, dtype=torch.float16)
+    _refused("share some", bergen_amd.kv_cache_write, k, k, slots, half[:2], half[1:])
+    two = torch.zeros(4, 3, 16, 32, dtype=torch.float16)
+    _refused("must be on the GPU", bergen_amd.kv_cache_write, k, k, slots, two[:2], two[2:])
+
+
 def test_attention_refusals():
     base = dict(q=torch.zeros(2, 6, 32, dtype=torch.bfloat16), block_table=torch.zeros(2, 4, dtype=torch.int32),
                 lengths=torch.zeros(2, dtype=torch.int32), **_cache_args())
