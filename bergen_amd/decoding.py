@@ -12,11 +12,13 @@ AutoModelForCausalLM, models/generators/llm.py).
   token_logprobs       log probabilities of given tokens, entropy, likeliest alternatives
 
 They take device tensors, ENQUEUE on the current stream of the tensors' device and return (the other entry points of this package wait); they can
-be captured into a graph.  They run inference only: a tensor that requires a gradient is refused while gradients are recorded.
+be captured into a graph.  They run inference only: a tensor that requires a gradient is refused while gradients are recorded,
+and one that carries a tangent (forward-mode differentiation).
 """
 import collections
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -41,9 +43,13 @@ def _fail(message):
 
 
 def _one_device(names, *tensors):
-    """Every tensor (None: not given) on one GPU, and none that waits for a gradient; -> that GPU's index.  names: theirs, for a refusal."""
+    """Every tensor (None: not given) on one GPU, and none that waits for a gradient or carries a tangent; -> that GPU's index.  names: theirs, for a refusal."""
     index = tensors[0].get_device()
     grad = torch.is_grad_enabled()
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():  # (inside forward_ad.dual_level(); under no_grad() too)
+        for name, t in zip(names.split(), tensors):
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                _fail(f"{name} carries a tangent and there is no derivative here")
     for t in tensors:
         if t is not None and (t.get_device() != index or (grad and t.requires_grad)):
             for name, t in zip(names.split(), tensors):

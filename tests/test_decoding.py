@@ -189,6 +189,31 @@ def test_a_gradient_is_refused_while_it_is_recorded():
         decoding._one_device("q k", torch.zeros(2), leaf)
 
 
+def test_a_tangent_is_refused():
+    """Forward-mode differentiation: requires_grad is False, and the tangent would be lost; under no_grad() it lives on, in inference mode it does not."""
+    import torch.autograd.forward_ad as fwd
+    a = _rotary_args()
+    x, t = torch.zeros(2, 9), torch.zeros(2, dtype=torch.int64)
+    with fwd.dual_level():
+        for name in ("q", "k"):
+            dual = {**a, name: fwd.make_dual(a[name], torch.ones_like(a[name]))}
+            assert not dual[name].requires_grad
+            for inplace in (False, True):
+                _refused(f"{name} carries a tangent", bergen_amd.qk_norm_rotary, **dual, inplace=inplace)
+            with torch.no_grad():
+                _refused(f"{name} carries a tangent", bergen_amd.qk_norm_rotary, **dual)
+            with torch.inference_mode():
+                _refused("must be on the GPU", bergen_amd.qk_norm_rotary, **dual)
+        w = fwd.make_dual(torch.ones(64), torch.ones(64))
+        _refused("k_weight carries a tangent", bergen_amd.qk_norm_rotary, **a, k_weight=w)
+        _refused("logits carries a tangent", bergen_amd.token_logprobs, fwd.make_dual(x, x), t)
+        c = _cache_args()
+        k, slots = torch.zeros(5, 3, 32), torch.zeros(5, dtype=torch.int64)
+        _refused("v carries a tangent", bergen_amd.kv_cache_write, k, fwd.make_dual(k.clone(), k), slots, **c)
+        _refused("v_scale carries a tangent", bergen_amd.kv_cache_read, slots, **{**c, "v_scale": fwd.make_dual(c["v_scale"], c["v_scale"].clone())})
+        _refused("must be on the GPU", bergen_amd.token_logprobs, x, t)
+
+
 def test_rotary_frequencies():
     f = bergen_amd.rotary_frequencies(8, 100.0, 0.5, device="cpu")
     assert f.dtype == torch.float64 and torch.allclose(f, 0.5 * torch.tensor([1, 100 ** -0.25, 0.1, 100 ** -0.75], dtype=torch.float64), rtol=1e-15)
