@@ -12,7 +12,7 @@ AutoModelForCausalLM, models/generators/llm.py).
   token_logprobs       log probabilities of given tokens, entropy, likeliest alternatives
 
 They take device tensors, ENQUEUE on the current stream of the tensors' device and return (the other entry points of this package wait); they can
-be captured into a graph.  They run inference only: a tensor that requires a gradient is refused while gradients are recorded,
+be captured into a graph, but not traced (torch.jit.trace).  They run inference only: a tensor that requires a gradient is refused while gradients are recorded,
 and one that carries a tangent (forward-mode differentiation).
 """
 import collections
@@ -46,6 +46,8 @@ def _one_device(names, *tensors):
     """Every tensor (None: not given) on one GPU, and none that waits for a gradient or carries a tangent; -> that GPU's index.  names: theirs, for a refusal."""
     index = tensors[0].get_device()
     grad = torch.is_grad_enabled()
+    if torch._C._get_tracing_state() is not None:
+        _fail("torch.jit.trace would record the outputs' memory and none of the work: these operators cannot be traced")
     if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():  # (inside forward_ad.dual_level(); under no_grad() too)
         for name, t in zip(names.split(), tensors):
             if t is not None and forward_ad.unpack_dual(t).tangent is not None:

@@ -214,6 +214,19 @@ def test_a_tangent_is_refused():
         _refused("must be on the GPU", bergen_amd.token_logprobs, x, t)
 
 
+@pytest.mark.filterwarnings("ignore")
+def test_a_trace_is_refused():
+    a, c = _rotary_args(), _cache_args()
+    k, slots = torch.zeros(5, 3, 32), torch.zeros(5, dtype=torch.int64)
+    q, table, n = torch.zeros(2, 6, 32, dtype=torch.bfloat16), torch.zeros(2, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    calls = [(lambda x: bergen_amd.qk_norm_rotary(**{**a, "q": x}), a["q"]), (lambda x: bergen_amd.token_logprobs(x, slots[:2]).logprobs, torch.zeros(2, 9)),
+             (lambda x: bergen_amd.kv_cache_write(x, k, slots, **c), k), (lambda x: bergen_amd.kv_cache_read(x, **c), slots),
+             (lambda x: bergen_amd.paged_attention(x, c["k_cache"], c["v_cache"], table, n, k_scale=c["k_scale"], v_scale=c["v_scale"]), q)]
+    for call, x in calls:
+        _refused("cannot be traced", torch.jit.trace, call, x)
+        _refused("must be on the GPU", call, x)
+
+
 def test_rotary_frequencies():
     f = bergen_amd.rotary_frequencies(8, 100.0, 0.5, device="cpu")
     assert f.dtype == torch.float64 and torch.allclose(f, 0.5 * torch.tensor([1, 100 ** -0.25, 0.1, 100 ** -0.75], dtype=torch.float64), rtol=1e-15)
