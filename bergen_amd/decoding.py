@@ -107,24 +107,39 @@ def _distinct(name, t):
         if size > 1:
             if not (stride >= room):
                 _fail(f"{name} overlaps itself (shape {tuple(t.shape)}, strides {t.stride()}): it cannot be written")
-            room = stride * size
+            room += stride * (size - 1)
+
+
+def _meet(at, a, b):
+    """Whether two lattices share an element: a and b, [(size, stride)] with the longest stride first, none overlapping itself, b's first element `at`
+    elements behind a's.  The rows of one that reach the other are looked at in turn, those of both by their difference where they are equally far apart."""
+    if not a and not b:
+        return at == 0
+    (n, step_a), (m, step_b) = (a or [(1, 0)])[0], (b or [(1, 0)])[0]
+    step = max(step_a, step_b)
+    rest_a, rest_b = a[1:] if step_a == step else a, b[1:] if step_b == step else b
+    reach_a, reach_b = (sum((size - 1) * by for size, by in x) for x in (rest_a, rest_b))
+    first, last = 1 - n if step_a == step else 0, m - 1 if step_b == step else 0  # b's row less a's
+    near = range(max(first, -((at + reach_b) // step)), min(last, (reach_a - at) // step) + 1)
+    return len(near) > 1000 or any(_meet(at + j * step, rest_a, rest_b) for j in near)
 
 
 def _apart(q, k):
-    """q's and k's memory does not meet: separate ranges, or separate columns of rows that are equally far apart."""
-    size = q.element_size()
+    """q's and k's memory does not meet: separate ranges, separate columns of rows that are equally far apart, or heads between each other's."""
     if 0 in q.shape or 0 in k.shape:
         return
     ends = [sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1 for t in (q, k)]
-    at = (k.data_ptr() - q.data_ptr()) // size
-    if at >= ends[0] or -at >= ends[1]:
+    at, off = divmod(k.data_ptr() - q.data_ptr(), q.element_size())
+    if at >= ends[0] or -at >= ends[1] + (off > 0):
         return
     row = q.stride(0)
-    if q.shape[0] > 1 and k.stride(0) == row:
+    if q.shape[0] > 1 and k.stride(0) == row and not off:
         cols = [e - (t.shape[0] - 1) * row for e, t in zip(ends, (q, k))]
         if at % row >= cols[0] and at % row + cols[1] <= row:
             return
-    _fail("q and k overlap: they cannot be written in place")
+    dims = [sorted(((n, st) for n, st in zip(t.shape, t.stride()) if n > 1), key=lambda p: -p[1]) for t in (q, k)]
+    if off or _meet(at, *dims):
+        _fail("q and k overlap: they cannot be written in place")
 
 
 def rotary_frequencies(rotary_dim, theta=10000.0, scale=1.0, device="cuda"):

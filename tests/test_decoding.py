@@ -53,6 +53,54 @@ def test_rotary_refusals(change, match):
     _refused(match, bergen_amd.qk_norm_rotary, **{**_rotary_args(), **change})
 
 
+def _views(*made):
+    buf = torch.zeros(4000, dtype=torch.bfloat16)
+    return [buf.as_strided(size, stride, 1000 + at) for size, stride, at in made]
+
+
+@pytest.mark.parametrize("q, k", [
+    (((5, 4, 16), (192, 48, 1), 0), ((5, 4, 16), (192, 48, 1), 16)),       # [tokens, heads, 3, dim]: queries and keys of each head side by side
+    (((5, 4, 16), (192, 48, 1), 16), ((5, 4, 16), (192, 48, 1), 0)),
+    (((5, 4, 16), (192, 48, 1), 0), ((5, 1, 16), (192, 48, 1), 32)),       # one key head between the queries' heads
+    (((5, 4, 16), (192, 48, 1), 0), ((5, 2, 16), (192, 96, 1), 64)),       # every other head
+    (((1, 4, 16), (7, 48, 1), 0), ((1, 4, 16), (9, 48, 1), 16)),
+    (((4, 5, 16), (16, 128, 1), 0), ((4, 5, 16), (16, 128, 1), 64)),       # heads first
+    (((3, 2, 8), (21, 10, 1), 0), ((3, 2, 2), (21, 10, 1), 8)),            # the last head ends in the next row's gap
+    (((2, 3, 1), (5, 2, 1), 0), ((2, 2, 1), (5, 2, 1), 1)),
+])
+def test_what_lies_between_may_be_written_in_place(q, k):
+    from bergen_amd import decoding
+    q, k = _views(q, k)
+    for t in (q, k):
+        decoding._distinct("q", t)
+    decoding._apart(q, k)
+    decoding._apart(k, q)
+
+
+def test_overlaps_are_found():
+    """All small lattices around each other: refused exactly where they share an element."""
+    import itertools
+    import random
+    from bergen_amd import decoding
+    rng, shared, apart = random.Random(0), 0, 0
+    for _ in range(4000):
+        d, h, t = rng.choice([1, 2, 3, 4]), rng.choice([1, 2, 3]), rng.choice([1, 2, 3, 4])
+        by_head = d * rng.choice([1, 1, 2, 3]) + rng.choice([0, 0, 1])
+        strides = (rng.choice([by_head * h, by_head * h + 1, 2 * by_head * h]), by_head, 1) if rng.random() < 0.8 else (d, d * t * rng.choice([1, 2]), 1)
+        other = strides if rng.random() < 0.7 else (strides[0], strides[1] * 2, 1)
+        q, k = _views(((t, h, d), strides, 0), ((t, rng.choice([1, h]), d), other, rng.randint(-30, 30)))
+        at = [{v.storage_offset() + sum(i * s for i, s in zip(x, v.stride())) for x in itertools.product(*map(range, v.shape))} for v in (q, k)]
+        if any(len(a) < v.numel() for a, v in zip(at, (q, k))):
+            continue
+        if at[0] & at[1]:
+            shared += 1
+            _refused("q and k overlap", decoding._apart, q, k)
+        else:
+            apart += 1
+            decoding._apart(q, k)
+    assert shared > 1000 and apart > 1000
+
+
 def _cache_args(dtype=torch.int8, pages=2, heads=3, page=16, dim=32):
     c = bergen_amd.kv_cache(pages, heads, page, dim, dtype, device="cpu")
     return dict(k_cache=c.k_cache, v_cache=c.v_cache, k_scale=c.k_scale, v_scale=c.v_scale)

@@ -70,6 +70,21 @@ def test_rotary_strides(dtype):
     check_rotary(shared[:, :6], shared[:, 6:], pos, f, w, w)
 
 
+@pytest.mark.parametrize("dtype, dim", [(BF, 64), (BF, 50), (F32, 64)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_in_place_between_heads(dtype, dim, interleaved):
+    """[tokens, heads, 3, dim]: each head's query, key and value side by side.  The values, and what a call on copies gives, stay as they are."""
+    g = gen(12)
+    f, pos, w = bergen_amd.rotary_frequencies(dim), torch.arange(9, device="cuda"), 1 + 0.1 * randn(g, dim, dtype=dtype)
+    x = randn(g, 9, 6, 3, dim, dtype=dtype)
+    want = bergen_amd.qk_norm_rotary(x[:, :, 0].contiguous(), x[:, :, 1].contiguous(), pos, f, w, w, interleaved=interleaved)
+    values = x[:, :, 2].clone()
+    check_rotary(x[:, :, 0], x[:, :, 1], pos, f, w, w, interleaved, inplace=True)
+    for i in (0, 1):
+        assert torch.equal(x[:, :, i], want[i])
+    assert torch.equal(x[:, :, 2], values)
+
+
 def test_rotary_far_positions_and_values():
     g = gen(4)
     f = bergen_amd.rotary_frequencies(128, theta=500000.0, scale=0.25)
