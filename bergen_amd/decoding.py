@@ -262,6 +262,8 @@ def kv_cache_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
                 if codes < scales + size_s and scales < codes + size:
                     _fail("the cache's codes and its scales share memory")
     device = _one_device("k v slots k_cache v_cache k_scale v_scale", k, v, slots, k_cache, v_cache, k_scale, v_scale)
+    if not pages:
+        pages, tokens = 1, 0  # every slot is outside it: the sizes are checked, nothing is written
     _call(device, _lib.lib().bh_op_kv_write, kp, k0, k1, vp, v0, v1, _FLOATS[k.dtype], slots.data_ptr(), tokens, heads, dim, kc, vc, _ptr(k_scale),
           _ptr(v_scale), _CACHES[k_cache.dtype], pages, page)
     torch.autograd.graph.increment_version([t for t in (k_cache, v_cache, k_scale, v_scale) if t is not None])
@@ -278,6 +280,9 @@ def kv_cache_read(slots, k_cache, v_cache, k_scale=None, v_scale=None, dtype=tor
     tokens = slots.shape[0]
     k = slots.new_empty((tokens, heads, dim), dtype=dtype)
     v = torch.empty_like(k)
+    if not pages:
+        pages, tokens = 1, 0
+        k.zero_(), v.zero_()
     _call(device, _lib.lib().bh_op_kv_read, k.data_ptr(), heads * dim, dim, v.data_ptr(), heads * dim, dim, _FLOATS[dtype], slots.data_ptr(), tokens,
           heads, dim, k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), _CACHES[k_cache.dtype], pages, page)
     return k, v
@@ -308,6 +313,8 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, scale=None, k_sca
     width, (t0, dense) = block_table.shape[1], block_table.stride()
     if dense != 1 and width > 1:
         _fail("block_table's rows must be dense")
+    if not pages:
+        width = 0  # no entry names a page of it
     if lengths.dtype != torch.int32 or lengths.dim() != 1 or lengths.shape[0] != batch or not lengths.is_contiguous():
         _fail(f"lengths must be contiguous int32 [{batch}]")
     if alibi_slopes is not None and (alibi_slopes.dim() != 1 or alibi_slopes.shape[0] != nq or alibi_slopes.dtype != torch.float32

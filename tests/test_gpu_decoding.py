@@ -226,6 +226,24 @@ def test_cache_slots_outside():
     assert bergen_amd.kv_cache_read(slots[:0], *c)[0].shape == (0, 2, 32)
 
 
+@pytest.mark.parametrize("cache", [BF, I8])
+def test_an_empty_cache(cache):
+    """No pages: every slot and every table entry is outside it.  Sizes are still checked."""
+    c = bergen_amd.kv_cache(0, 2, 16, 64, cache)
+    k, slots = torch.ones(3, 2, 64, dtype=BF, device="cuda"), torch.tensor([0, -1, 5], device="cuda")
+    bergen_amd.kv_cache_write(k, k, slots, *c)
+    for x in bergen_amd.kv_cache_read(slots, *c):
+        assert x.shape == (3, 2, 64) and not x.any()
+    q, n = torch.ones(2, 4, 64, dtype=BF, device="cuda"), torch.tensor([5, 0], dtype=torch.int32, device="cuda")
+    out, lse = bergen_amd.paged_attention(q, c.k_cache, c.v_cache, torch.zeros(2, 300, dtype=torch.int32, device="cuda"), n, k_scale=c.k_scale,
+                                          v_scale=c.v_scale, return_lse=True)
+    assert not out.any() and (lse == -math.inf).all()
+    c = bergen_amd.kv_cache(0, 2, 12, 64, cache)
+    for call in (lambda: bergen_amd.kv_cache_write(k, k, slots, *c), lambda: bergen_amd.kv_cache_read(slots, *c)):
+        with pytest.raises(RuntimeError, match="page_size 12"):
+            call()
+
+
 def test_cache_strides():
     g = gen(2)
     qkv = randn(g, 6, 7, 48, dtype=BF)
