@@ -104,6 +104,14 @@ __device__ __forceinline__ float over_groups_sum(float v) {
     return v + __shfl_xor(v, 32);
 }
 
+// the power of two at or above v >= 0, 2^126 at most
+__device__ __forceinline__ float power_above(float v) {
+    const unsigned b = __float_as_uint(v);
+    return b > 0x7e800000u ? 0x1p126f : __uint_as_float((b + 0x7fffffu) & 0x7f800000u);
+}
+// 2^n / p, p a power of two between 2^(n - 126) and 2^126
+__device__ __forceinline__ float over_power(int n, float p) { return __uint_as_float(((unsigned)(254 + n) << 23) - __float_as_uint(p)); }
+
 // two codes of a word, the lower two or (which = 1) the upper two, as two fp16
 template <int CACHE>
 __device__ __forceinline__ unsigned two_f16(unsigned word, int which) {
@@ -133,6 +141,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : DP == 64 ? 4 : EXA
     constexpr int VW = NJ * ES / 4;               // their words
     constexpr bool F16 = std::is_same<M, _Float16>::value;
     constexpr float HOLD = F16 ? 14.f : 0.f;      // weights are held times 2^HOLD
+    constexpr float LEAST = 0x1p-112f;            // least unit of the values' scales times weights: 2^HOLD over it is finite, and a scale of 2^-126 keeps all its bits
 
     __shared__ frag sh_q[KS][64];  // registers are short; each wave writes the same and reads what it wrote
     __shared__ float sh_stats[WAVES][2][16];
@@ -199,8 +208,11 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : DP == 64 ? 4 : EXA
     }
     const float cap = a.softcap * LOG2E, cap_unit = a.softcap > 0.f ? 2.f / a.softcap : 0.f;
 
-    float m, total;  // of head n: the same m in its 4 lanes; each lane's own sum, times 2^HOLD
-    float v_top;     // values' scales are held against a power of two
+    float m, total;  // of head n: the same m in its 4 lanes; each lane's own sum, times 2^HOLD (scaled: as it is)
+    // scaled: a power of two for head n that o and the held products (weight times value's scale) count in: no product is above it when it is held,
+    // and their largest not far below it, however the scales compare (counting in the scales alone gave 0 beside values of 1e12 that weigh e^-100;
+    // this costs a steep distance bias 0.8 us of 44).  slack: what the weights have lost since it was set
+    float unit_v, slack;
     floatx4 o[NJ];
 
     const int* table = a.table + seq * a.table_stride;
@@ -285,7 +297,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : DP == 64 ? 4 : EXA
     // more with hi alone, for those sums only
     bool both = true;
     for (;; both = false) {
-        m = -INFINITY, total = 0.f, v_top = 0x1p-126f;
+        m = -INFINITY, total = 0.f, unit_v = LEAST, slack = 1.f;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) o[j] = floatx4{0.f, 0.f, 0.f, 0.f};
         int t0 = lo + wave * TILE;
@@ -382,30 +394,43 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : DP == 64 ? 4 : EXA
                 const float fade = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - now);
                 m = now;
                 total *= fade;
+                float by = fade;
+                if constexpr (SCALED) {
+                    slack *= fade;
+                    if (__any(slack < 0x1p-12f)) {  // (a large scale whose weight is gone must not hide the ones to come; 2^14 - 12 and hi + lo still keep 2^-27)
+                        const float to = fmaxf(LEAST, power_above(unit_v * slack));
+                        by = unit_v * fade * over_power(0, to);  // at most 2^12: o is in 32 bits
+                        unit_v = to, slack = 1.f;
+                    }
+                }
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) o[j] *= fade;
+                for (int j = 0; j < NJ; ++j) o[j] *= by;
             }
-            if constexpr (SCALED) {
-                float big = fabsf(vs[0]);
+            const float base = m == -INFINITY ? 0.f : SCALED ? m : m - HOLD;
 #pragma unroll
-                for (int r = 1; r < 8; ++r) big = fmaxf(big, fabsf(vs[r]));
-                if (__any(big > v_top)) {
-                    // the power of two at or above the largest scale of the wave's tokens so far
-                    const unsigned b = __float_as_uint(over_groups_max(big));
-                    const float up = __uint_as_float((b & 0x7f800000u) + ((b & 0x7fffffu) && b < 0x7f000000u ? 0x800000u : 0u));
-                    const float to = fmaxf(v_top, up), shrink = v_top / to;
+            for (int r = 0; r < 8; ++r) {
+                x[r] = __builtin_amdgcn_exp2f(x[r] - base);
+                total += x[r];
+                if constexpr (SCALED) x[r] *= vs[r];
+            }
+            float per = 1.f;
+            if constexpr (SCALED) {
+                float big = fabsf(x[0]);
+#pragma unroll
+                for (int r = 1; r < 8; ++r) big = fmaxf(big, fabsf(x[r]));
+                if (__any(big > unit_v)) {
+                    const float to = fmaxf(unit_v, power_above(over_groups_max(big))), shrink = unit_v * over_power(0, to);
 #pragma unroll
                     for (int j = 0; j < NJ; ++j) o[j] *= shrink;
-                    v_top = to;
+                    slack = to > unit_v ? 1.f : slack;
+                    unit_v = to;
                 }
+                per = over_power(14, unit_v);
             }
-            const float base = m == -INFINITY ? 0.f : m - HOLD, per = 1.f / v_top;
             frag hi_p, lo_p;
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
-                float p = __builtin_amdgcn_exp2f(x[r] - base);
-                total += p;
-                if constexpr (SCALED) p *= vs[r] * per;
+                float p = SCALED ? x[r] * per : x[r];
                 // one value for both: left alone, the compiler rounds the product above to fp16 once in a fused instruction for hi and once
                 // by way of fp32 for what hi is subtracted from, and where those fall on different sides lo belongs to another hi
                 asm("" : "+v"(p));
@@ -470,7 +495,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : DP == 64 ? 4 : EXA
 #pragma unroll
             for (int r = 0; r < 4; ++r) sh_out[wave][n][NJ * (4 * g + r) + j] = o[j][r];
     }
-    total *= F16 ? 0x1p-14f : 1.f;
+    total *= F16 && !SCALED ? 0x1p-14f : 1.f;
 
     // ---- the workgroup's waves joined
     total = over_groups_sum(total);
@@ -483,7 +508,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : DP == 64 ? 4 : EXA
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) all = fmaxf(all, sh_stats[w][0][n]);
     const float base = all == -INFINITY ? 0.f : all;
-    const float mine = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - base - HOLD) * (SCALED ? v_top : 1.f);
+    const float mine = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - base - HOLD) * (SCALED ? unit_v : 1.f);
     // lane (g, n), tile j, element r: head n, dim NJ (4 g + r) + j
 #pragma unroll
     for (int j = 0; j < NJ; ++j)

@@ -448,6 +448,30 @@ def test_attention_scales_of_values(size):
         check_attention(q, c, table, [311], scale=1e-9)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("cache", [I8, E4])
+@pytest.mark.parametrize("far", [1e6, 1e12, 1e25, 1e-25])
+def test_attention_of_large_values_without_weight(cache, dim, far):
+    """8-bit values that are far larger than those that count (or far smaller) and weigh next to nothing: the distance bias leaves e^-100 and less of
+    the tokens before the last 100, and in the last sequence a score of its own decides."""
+    g = gen(dim)
+    lengths = [400, 130, 1500, 300]
+    pages = sum(-(-n // 16) for n in lengths)
+    c = bergen_amd.kv_cache(pages, 2, 16, dim, cache)
+    rows = pages * 16
+    table = table_for(g, lengths, 16, pages, 0)
+    k, v = torch.zeros(rows, 2, dim, device="cuda"), randn(g, rows, 2, dim)
+    for b, n in enumerate(lengths):
+        t = torch.arange(n, device="cuda")
+        slot = table[b].long()[t // 16] * 16 + t % 16
+        v[slot[: max(0, n - 110)]] *= far
+        if b == 3:
+            k[slot[7]], v[slot[7]] = 300.0, 1.0
+    bergen_amd.kv_cache_write(k, v, torch.arange(rows, device="cuda"), *c)
+    q = torch.ones(4, 8, dim, dtype=BF, device="cuda")
+    check_attention(q, c, table, lengths, slopes=torch.linspace(1.0, 1.5, 8, device="cuda"))
+
+
 def test_attention_far_into_a_cache():
     """Offsets past 2^31 bytes: 8-bit pages at the end of a cache of 2.5 GB each for keys and values."""
     g = gen(8)
