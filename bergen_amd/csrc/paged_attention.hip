@@ -130,7 +130,7 @@ __device__ __forceinline__ unsigned two_f16(unsigned word, int which) {
 // E: the queries' type; CACHE: BH_F16 / BH_BF16 (E's own), BH_I8, BH_E4M3; DP: head dim, rounded up to 64, 128 or 256 (EXACT: is it).
 // ONE_PAGE: pages of 32 tokens and more, so that a tile lies in one.
 template <typename E, int CACHE, int DP, bool EXACT, bool ONE_PAGE>
-__global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : DP == 64 ? 4 : EXACT ? 3 : 2) bh_paged_attention_kernel(PagedArgs a) {
+__global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : DP == 64 ? 4 : EXACT || CACHE == BH_I8 || CACHE == BH_E4M3 ? 3 : 2) bh_paged_attention_kernel(PagedArgs a) {
     constexpr bool SCALED = CACHE == BH_I8 || CACHE == BH_E4M3;
     typedef typename std::conditional<SCALED, _Float16, E>::type M;  // the MFMAs' type
     typedef typename Mma<M>::frag frag;
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : DP == 64 ? 4 : EXA
     float m, total;  // of head n: the same m in its 4 lanes; each lane's own sum, times 2^HOLD (scaled: as it is)
     // scaled: a power of two for head n that o and the held products (weight times value's scale) count in: no product is above it when it is held,
     // and their largest not far below it, however the scales compare (counting in the scales alone gave 0 beside values of 1e12 that weigh e^-100;
-    // this costs a steep distance bias 0.8 us of 44).  slack: what the weights have lost since it was set
+    // this costs a steep distance bias 1.6 us of 44, heads of 256 2 %).  slack: what the weights have lost since it was set
     float unit_v, slack;
     floatx4 o[NJ];
 
@@ -413,6 +413,9 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : DP == 64 ? 4 : EXA
                 total += x[r];
                 if constexpr (SCALED) x[r] *= vs[r];
             }
+            // (the sum now, not when there is time for it: the weights would wait beside the products, and 8-bit heads of 80, 96 and 112 have no registers
+            // for both in 3 waves a SIMD: 64 sequences of 4000 tokens, 8 key heads of 96, e4m3: 73 us, 85 in 2 waves.  Heads of 64 lose 5 of 45 us by it)
+            if constexpr (SCALED && DP == 128 && !EXACT) asm volatile("" : "+v"(total));
             float per = 1.f;
             if constexpr (SCALED) {
                 float big = fabsf(x[0]);

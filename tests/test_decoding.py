@@ -221,6 +221,33 @@ def test_refused_by_the_c_entry_points():
     assert lib.bh_op_token_logprobs_workspace(1, 100, F, 101) == E
 
 
+def test_registers_as_the_makefile_builds():
+    """The decoding operators' kernels with their own flags: nothing in scratch, and 8-bit attention of heads up to 128 in 3 waves a SIMD (of 64: 4)."""
+    import os
+    import re
+    import subprocess
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "bergen_amd", "csrc")
+    jobs = []
+    for src in ("decode_ops", "paged_attention", "token_logprobs"):
+        line = [w for w in subprocess.run(["make", "-n", "-W", f"{src}.hip", f"../lib/obj/{src}.o"], cwd=csrc, capture_output=True, text=True, check=True).stdout.splitlines()
+                if f"-c {src}.hip" in w][0].split()
+        assert "-packed-fp32-ops" in line
+        jobs.append(subprocess.Popen(line[: line.index("-o")] + ["-o", os.devnull, "-Rpass-analysis=kernel-resource-usage"], cwd=csrc, stderr=subprocess.PIPE, text=True))
+    seen = 0
+    for job in jobs:
+        text = job.communicate()[1]
+        assert job.returncode == 0, text[-2000:]
+        for block in text.split("Function Name: ")[1:]:
+            name = block.split()[0]
+            value = {k.strip(): int(v) for k, v in re.findall(r"remark:\s+([A-Za-z ]+?)(?: \[[^\]]*\])?: (\d+)", block)}
+            seen += 1
+            assert value["ScratchSize"] == 0 and value["VGPRs Spill"] == 0, (name, value)
+            form = re.search(r"bh_paged_attention_kernelIDF16.Li([34])ELi(64|128)E", name)
+            if form:
+                assert value["Occupancy"] >= {"64": 4, "128": 3}[form.group(2)], (name, value)
+    assert seen > 60
+
+
 def test_older_entry_points_still_refuse_the_new_types():
     lib = _lib.lib()
     h = ctypes.c_void_p()
