@@ -16,8 +16,8 @@
 //   O^T += V^T P^T  wants in lane (g, n) the weights of 8 tokens of head n: those 8, as they are.  Its V^T operand, lane (g, i),
 //                   wants the same 8 tokens of one dim; the lane loads D / 16 consecutive dims of each of them (a group's 16 lanes: a
 //                   whole row) and turns its own little block round with byte permutes.
-// Keys: lane (g, i) loads 16 bytes of its row, groups side by side.  8-bit codes become fp16, exactly, between load and
-// MFMA; the keys' scale multiplies the score, the values' scale the weight.
+// Keys: lane (g, i) loads 16 bytes of its row, groups side by side.  8-bit codes become numbers of the queries' type, and values fp16, exactly, between
+// load and MFMA; the keys' scale multiplies the score, the values' scale the weight.
 // Weights reach the MFMA as a sum of two numbers of its type (hi + lo): bf16 alone would keep 2^-8 of a weight, as much as
 // the output's own rounding.  fp16 weights are held times 2^14 so that small ones do not become subnormal.
 //
@@ -127,13 +127,26 @@ __device__ __forceinline__ unsigned two_f16(unsigned word, int which) {
                  : __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.0f, false));
 }
 
+// the same as two of the queries' type: codes have at most 8 significant bits, which bf16 keeps as well
+template <typename E, int CACHE>
+__device__ __forceinline__ unsigned two_keys(unsigned word, int which) {
+    if constexpr (std::is_same<E, _Float16>::value) return two_f16<CACHE>(word, which);
+    if constexpr (CACHE == BH_E4M3)
+        return which ? __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, 1.0f, true))
+                     : __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, 1.0f, false));
+    // a code as fp32 ends in 16 zero bits: its upper half is the bf16
+    const float lo = (float)(int)__builtin_amdgcn_sbfe((int)word, which ? 16 : 0, 8), hi = (float)(int)__builtin_amdgcn_sbfe((int)word, which ? 24 : 8, 8);
+    return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+
 // E: the queries' type; CACHE: BH_F16 / BH_BF16 (E's own), BH_I8, BH_E4M3; DP: head dim, rounded up to 64, 128 or 256 (EXACT: is it).
 // ONE_PAGE: pages of 32 tokens and more, so that a tile lies in one.
 template <typename E, int CACHE, int DP, bool EXACT, bool ONE_PAGE>
 __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : DP == 64 ? 4 : EXACT || CACHE == BH_I8 || CACHE == BH_E4M3 ? 3 : 2) bh_paged_attention_kernel(PagedArgs a) {
     constexpr bool SCALED = CACHE == BH_I8 || CACHE == BH_E4M3;
-    typedef typename std::conditional<SCALED, _Float16, E>::type M;  // the MFMAs' type
+    typedef typename std::conditional<SCALED, _Float16, E>::type M;  // the type of the weights' and values' MFMAs; the scores' is E
     typedef typename Mma<M>::frag frag;
+    typedef typename Mma<E>::frag key_frag;
     constexpr int ES = SCALED ? 1 : 2;            // bytes of a cached element
     constexpr int KS = DP / 32;                   // steps of S^T
     constexpr int KL = KS * 8 * ES / 16;          // 16-byte loads of a key row per lane
@@ -143,7 +156,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : DP == 64 ? 4 : EXA
     constexpr float HOLD = F16 ? 14.f : 0.f;      // weights are held times 2^HOLD
     constexpr float LEAST = 0x1p-112f;            // least unit of the values' scales times weights: 2^HOLD over it is finite, and a scale of 2^-126 keeps all its bits
 
-    __shared__ frag sh_q[KS][64];  // registers are short; each wave writes the same and reads what it wrote
+    __shared__ key_frag sh_q[KS][64];  // registers are short; each wave writes the same and reads what it wrote
     __shared__ float sh_stats[WAVES][2][16];
     __shared__ float sh_out[WAVES][16][DP + 4];
 
@@ -168,8 +181,8 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : DP == 64 ? 4 : EXA
     float unit = a.scale * LOG2E;  // of a score, in powers of two
     {
         float top = 0.f;
-        bf16x8 qb[KS];
-        (void)qb;
+        key_frag qs[KS];
+        (void)qs;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int d = SCALED ? 16 * ((s >> 1) * 4 + g) + 8 * (s & 1) : 8 * (4 * s + g);
@@ -177,25 +190,26 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : DP == 64 ? 4 : EXA
             vec x = {};
             if (head_live && d < a.dim) x = *reinterpret_cast<const vec*>(qp + d);
             if constexpr (std::is_same<E, M>::value) {
-                sh_q[s][lane] = __builtin_bit_cast(frag, x);
+                sh_q[s][lane] = x;
             } else {
-                qb[s] = x;
+                qs[s] = x;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf((float)x[e]));
             }
         }
         if constexpr (!std::is_same<E, M>::value) {
-            // bf16 queries against 8-bit keys: as fp16, times the power of two that brings the head's largest to 2^7..2^8 (exact above
-            // 2^-22 of it)
+            // bf16 queries against 8-bit keys: times the power of two that brings the head's largest to 2^7..2^8, exact but below 2^-133 of it.  The
+            // codes are as large as the scales make them, and the sum of products with them must not leave fp32's range.  (As fp16, like the weights,
+            // the elements of a head whose largest is 2^24 times theirs and more would lose bits)
             top = over_groups_max(top);
             int e = (int)(__float_as_uint(top) >> 23) - 127;
             e = e > 126 ? 126 : e < -112 ? -112 : e;
             const float up = ldexpf(1.f, 7 - e);
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                frag f;
+                key_frag f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) f[i] = (_Float16)((float)qb[s][i] * up);
+                for (int i = 0; i < 8; ++i) f[i] = (E)((float)qs[s][i] * up);
                 sh_q[s][lane] = f;
             }
             unit *= ldexpf(1.f, e - 7);
@@ -332,16 +346,16 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : DP == 64 ? 4 : EXA
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
-                    frag kf;
+                    key_frag kf;
                     if constexpr (SCALED) {
                         const uint4 c = kr[u][s >> 1];
                         const unsigned w0 = s & 1 ? c.z : c.x, w1 = s & 1 ? c.w : c.y;
-                        const uint4 f = {two_f16<CACHE>(w0, 0), two_f16<CACHE>(w0, 1), two_f16<CACHE>(w1, 0), two_f16<CACHE>(w1, 1)};
-                        kf = __builtin_bit_cast(frag, f);
+                        const uint4 f = {two_keys<E, CACHE>(w0, 0), two_keys<E, CACHE>(w0, 1), two_keys<E, CACHE>(w1, 0), two_keys<E, CACHE>(w1, 1)};
+                        kf = __builtin_bit_cast(key_frag, f);
                     } else {
-                        kf = __builtin_bit_cast(frag, kr[u][s]);
+                        kf = __builtin_bit_cast(key_frag, kr[u][s]);
                     }
-                    st[u] = Mma<M>::mul(kf, sh_q[s][q_lane], st[u]);
+                    st[u] = Mma<E>::mul(kf, sh_q[s][q_lane], st[u]);
                 }
             float x[8];
 #pragma unroll

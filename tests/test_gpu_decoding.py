@@ -472,6 +472,31 @@ def test_attention_of_large_values_without_weight(cache, dim, far):
     check_attention(q, c, table, lengths, slopes=torch.linspace(1.0, 1.5, 8, device="cuda"))
 
 
+@pytest.mark.parametrize("dim", [64, 80, 128, 256])
+@pytest.mark.parametrize("cache", [I8, E4])
+@pytest.mark.parametrize("large", [2.0 ** 20, 2.0 ** 26, 2.0 ** 40])
+def test_attention_of_queries_with_a_large_element(cache, dim, large):
+    """bf16 queries whose largest element meets zeros in the keys: the scores are the small elements' alone."""
+    g = gen(dim)
+    lengths = [1, 40, 333]
+    c = bergen_amd.kv_cache(40, 2, 16, dim, cache)
+    k = randn(g, 640, 2, dim)
+    k[:, :, 5] = 0
+    bergen_amd.kv_cache_write(k, randn(g, 640, 2, dim), torch.arange(640, device="cuda"), *c)
+    q = 3 * randn(g, 3, 4, dim, dtype=BF)
+    q[:, :3, 5] = torch.tensor([large, -large, large / 8], device="cuda").to(BF)  # (the fourth head has none)
+    check_attention(q, c, table_for(g, lengths, 16, 40), lengths)
+    bad = q.clone()
+    bad[1, 0, 7], bad[2, 1, 9] = math.inf, math.nan                               # infinite and NaN elements stay with their head
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    table = table_for(gen(1), lengths, 16, 40)
+    want, got = (bergen_amd.paged_attention(x, c.k_cache, c.v_cache, table, n, k_scale=c.k_scale, v_scale=c.v_scale) for x in (q, bad))
+    assert torch.isnan(got[1, 0]).all() and torch.isnan(got[2, 1]).all()
+    keep = torch.ones(3, 4, dtype=torch.bool)
+    keep[1, 0] = keep[2, 1] = False
+    assert torch.equal(got.cpu()[keep], want.cpu()[keep])
+
+
 def test_attention_far_into_a_cache():
     """Offsets past 2^31 bytes: 8-bit pages at the end of a cache of 2.5 GB each for keys and values."""
     g = gen(8)
