@@ -32,10 +32,9 @@ _ready = set()
 
 # the current stream's handle: current_stream() builds an object around it, which takes longer than the launch it is wanted for
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
-
-
 # (likewise: the index without the question whether CUDA is initialised, which a tensor on the GPU has answered)
 _current = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_tracing = torch._C._get_tracing_state
 
 
 def _fail(message):
@@ -46,7 +45,7 @@ def _one_device(names, *tensors):
     """Every tensor (None: not given) on one GPU, and none that waits for a gradient or carries a tangent; -> that GPU's index.  names: theirs, for a refusal."""
     index = tensors[0].get_device()
     grad = torch.is_grad_enabled()
-    if torch._C._get_tracing_state() is not None:
+    if _tracing() is not None:
         _fail("torch.jit.trace would record the outputs' memory and none of the work: these operators cannot be traced")
     if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():  # (inside forward_ad.dual_level(); under no_grad() too)
         for name, t in zip(names.split(), tensors):
@@ -250,23 +249,23 @@ def kv_cache_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
     if slots.dtype != torch.int64 or slots.dim() != 1 or slots.shape[0] != tokens or not slots.is_contiguous():
         _fail(f"slots must be contiguous int64 [{tokens}]")
     kc, vc = k_cache.data_ptr(), v_cache.data_ptr()
-    size = k_cache.numel() * k_cache.element_size()
+    vectors = pages * heads * page
+    size = vectors * dim * (1 if scaled else 2)
     if kc < vc + size and vc < kc + size:
         _fail("k_cache and v_cache are the same memory, or share some")
+    ks = vs = None
     if scaled:
-        ks, vs, size_s = k_scale.data_ptr(), v_scale.data_ptr(), 4 * k_scale.numel()
+        ks, vs, size_s = k_scale.data_ptr(), v_scale.data_ptr(), 4 * vectors
         if ks < vs + size_s and vs < ks + size_s:
             _fail("k_scale and v_scale are the same memory, or share some")
-        for codes in (kc, vc):
-            for scales in (ks, vs):
-                if codes < scales + size_s and scales < codes + size:
-                    _fail("the cache's codes and its scales share memory")
+        if kc - size_s < ks < kc + size or kc - size_s < vs < kc + size or vc - size_s < ks < vc + size or vc - size_s < vs < vc + size:
+            _fail("the cache's codes and its scales share memory")
     device = _one_device("k v slots k_cache v_cache k_scale v_scale", k, v, slots, k_cache, v_cache, k_scale, v_scale)
     if not pages:
         pages, tokens = 1, 0  # every slot is outside it: the sizes are checked, nothing is written
-    _call(device, _lib.lib().bh_op_kv_write, kp, k0, k1, vp, v0, v1, _FLOATS[k.dtype], slots.data_ptr(), tokens, heads, dim, kc, vc, _ptr(k_scale),
-          _ptr(v_scale), _CACHES[k_cache.dtype], pages, page)
-    torch.autograd.graph.increment_version([t for t in (k_cache, v_cache, k_scale, v_scale) if t is not None])
+    _call(device, _lib.lib().bh_op_kv_write, kp, k0, k1, vp, v0, v1, _FLOATS[k.dtype], slots.data_ptr(), tokens, heads, dim, kc, vc, ks, vs,
+          _CACHES[k_cache.dtype], pages, page)
+    torch.autograd.graph.increment_version((k_cache, v_cache, k_scale, v_scale) if scaled else (k_cache, v_cache))
 
 
 def kv_cache_read(slots, k_cache, v_cache, k_scale=None, v_scale=None, dtype=torch.bfloat16):
