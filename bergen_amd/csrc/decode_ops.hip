@@ -6,7 +6,9 @@
 // passes through LDS; they need whole pieces and 16-byte rows.  Everything else (odd D, unaligned views) runs on the narrow
 // kernels: one wave per vector, one element per lane and step.
 // Bound: HBM (each element is read once and written once).  Measured: norm + rotary of 16384 tokens of 32 + 8 heads of 128, bf16: 68 us = 4.9 TB/s (a copy: 4.9);
-// 8192 such tokens in fp32: 62 us = 5.4 TB/s; 65536 tokens of 8 heads of 128 read from an e4m3 cache of 64-token pages as bf16: 70 us = 5.8 TB/s; 8192 written: 15 us.
+// 8192 such tokens in fp32, pairs side by side: 65 us = 5.1 TB/s; 65536 tokens of 8 heads of 128 read from an e4m3 cache of 64-token pages as bf16: 70 us = 5.8
+// TB/s; 8192 written: 17 us = 3.0 TB/s, most of it waiting (a group of lanes moves one vector and ends).  Rows that the narrow kernels take, 4096 tokens of
+// 32 + 8 heads of 100 in bf16: 50 us where a copy takes 13.
 #include "bh_decode.h"
 
 namespace {
@@ -200,8 +202,8 @@ __global__ void __launch_bounds__(256) bh_qk_norm_rotary_any_kernel(RotaryArgs a
                 if (d < a.dim) x[n] *= r * (a.w32 ? static_cast<const float*>(w)[d] : (float)static_cast<const E*>(w)[d]);
             }
         }
-        // the partner of element d sits in another lane and step: by way of LDS, the wave's own (16 exchanges between lanes took 56 us for 4096
-        // tokens of 32 heads of 100; this 42)
+        // the partner of element d sits in another lane and step: by way of LDS, the wave's own (16 exchanges between lanes took a
+        // third longer)
         float o[4];
         float* mine = vec[threadIdx.x >> 6];
 #pragma unroll

@@ -6,9 +6,10 @@
 // Bound: HBM, by the cache's bytes — each key and value is read once for the whole group of query heads that shares it.  A query
 // head alone makes 1 flop per byte, a group of 8 makes 8; on the vector units 8 would already take all their cycles, so both products run
 // on the matrix cores, 16 heads wide whether there are 16 or 1 (the matrix pipe is busy 5 % of the time for 4 heads a group in bf16).
-// Measured: 64 sequences of 90..8191 tokens, 8 key heads of 128, bf16: 186 us = 5.8 TB/s (the loads alone: 189 us); 3 of 100001..131072 tokens, e4m3: 145 us
-// = 5.0 TB/s (the loads alone: 135 us); 37 of 1..6000, window 4096, 12 heads of 64 without groups, int8: 44 us = 3.7 TB/s (the loads alone 31 us: the
-// vector instructions of a tile are the same for 1 head as for 16).
+// Measured: 64 sequences of 90..8191 tokens, 8 key heads of 128, bf16: 186 us = 5.8 TB/s (the loads alone take as long); 3 of 100001..131072 tokens, e4m3:
+// 126 us = 5.8 TB/s on some cards, 145 on others; 37 of 1..6000, window 4096, 12 heads of 64 without groups, int8: 43 us = 3.7 TB/s (the loads alone 31 us: the
+// vector instructions of a tile are the same for 1 head as for 16).  64 of 90..4095, 8 key heads of 256: 253 us in bf16, 139 in e4m3 (4.3 and 4.0 TB/s, one
+// wave a SIMD: registers); of 96: 92 and 47.
 //
 // A wave takes 32 tokens of one key head at a time and needs no LDS for them:
 //   S^T = K Q^T     two tiles of 16 tokens.  Row i of tile u is token 8 (i / 4) + 4 u + i % 4, so that lane (g, n) — g = lane / 16,
@@ -18,8 +19,9 @@
 //                   whole row) and turns its own little block round with byte permutes.
 // Keys: lane (g, i) loads 16 bytes of its row, groups side by side.  8-bit codes become numbers of the queries' type, and values fp16, exactly, between
 // load and MFMA; the keys' scale multiplies the score, the values' scale the weight.
-// Weights reach the MFMA as a sum of two numbers of its type (hi + lo): bf16 alone would keep 2^-8 of a weight, as much as
-// the output's own rounding.  fp16 weights are held times 2^14 so that small ones do not become subnormal.
+// Weights reach the MFMA as a sum of two numbers of its type (hi + lo): bf16 alone would keep 2^-8 of a weight, as much as the output's own rounding;
+// two keep 2^-17 (a third, the whole weight, costs 1 % of the time).  fp16 weights (8-bit caches: their products with the values' scales) are held times 2^14 so
+// that small ones do not become subnormal: two keep 2^-22 of them, and leave out 2^-39 of the sequence's largest.
 //
 // Pages are 8..1024 tokens (a power of two): 8 consecutive tokens share one.  A table entry outside [0, pages) names a page that is
 // not there: its tokens are left out.  What lies behind a sequence's end is neither counted nor multiplied (its values
@@ -225,7 +227,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : DP == 64 ? 4 : EXA
     float m, total;  // of head n: the same m in its 4 lanes; each lane's own sum, times 2^HOLD (scaled: as it is)
     // scaled: a power of two for head n that o and the held products (weight times value's scale) count in: no product is above it when it is held,
     // and their largest not far below it, however the scales compare (counting in the scales alone gave 0 beside values of 1e12 that weigh e^-100;
-    // this costs a steep distance bias 1.6 us of 44, heads of 256 2 %).  slack: what the weights have lost since it was set
+    // this costs a steep distance bias 1.2 us of 42, heads of 256 2 %).  slack: what the weights have lost since it was set
     float unit_v, slack;
     floatx4 o[NJ];
 

@@ -10,8 +10,9 @@
 // -inf (banned tokens) carries no probability; a row of nothing else has log probabilities -inf and entropy 0.  A row that holds a
 // NaN or +inf has NaN log probabilities and entropy; its alternatives are ordered with NaN below -inf.  Ties go to the lower index.
 // Bound: HBM and the vector units alike: a logit takes 9.2 of their issue slots (its exponential 4), which is as long as 2 bytes take from HBM.
-// Measured, 4096 rows of 128000 in bf16: 162 us = 6.5 TB/s without alternatives, 220 us with 8, 275 with 20 (the candidates' instructions; about
-// 30 of each wave's 32000 for 8).  61 rows of 120064, 20 alternatives: 16 + 8 us, 7 + 3 without; one row of 30522 in fp32, 5: 7 + 5 us (latency).
+// Measured, 4096 rows of 128000 in bf16: 164 us = 6.4 TB/s without alternatives, 201 us with 8, 247 with 20 (the candidates' instructions; about
+// 30 of each wave's 32000 for 8; in the first 10 ms of a load, while the card's clock settles, up to 290 with 8).  61 rows of 120064, 20 alternatives: 16 + 8 us
+// (the first step's candidates go in one by one, in an order that the join makes anew), 8 + 4 without; one row of 30522 in fp32, 5: 7 + 5 us (latency).
 #include "bh_decode.h"
 
 namespace {

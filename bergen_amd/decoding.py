@@ -202,7 +202,10 @@ KVCache = collections.namedtuple("KVCache", "k_cache v_cache k_scale v_scale")
 
 
 def kv_cache(pages, heads, page_size, dim, dtype=torch.bfloat16, device="cuda"):
-    """An empty paged cache -> KVCache(k_cache, v_cache [pages, heads, page_size, dim], k_scale, v_scale [pages, heads, page_size] or None)."""
+    """An empty paged cache -> KVCache(k_cache, v_cache [pages, heads, page_size, dim], k_scale, v_scale [pages, heads, page_size] or None).
+
+    The operators take page sizes that are a power of two, 8 .. 1024, and dim up to 256 (`paged_attention`: multiples of 16).
+    """
     if not (dtype in _CACHES):
         _fail(f"a cache holds float16, bfloat16, int8 or float8_e4m3fn, got {dtype}")
     shape = (pages, heads, page_size, dim)
