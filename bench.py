@@ -1714,12 +1714,29 @@ def run(args, env):
             except Exception as exc:
                 out["cpu_baseline"] = {"value": None, "unit": "queries/s", "cores": bergen_amd.utils.cpu_budget(), "kind": "port", "sample": "failed: " + repr(exc)}
         out["roofline"]["secondary"] = secondary_summary(out)
-        print(json.dumps(out), flush=True)
+        print("[bench] every leg in full: " + json.dumps(out), file=sys.stderr, flush=True)
+        print(json.dumps(bench_line(out)), flush=True)
     stage.close()
     if world > 1:
         dist.destroy_process_group()
     if rank == 0 and parity == "FAIL":
         sys.exit(3)
+
+
+WHOLE_IN_THE_LINE = ("metric", "value", "unit", "n_gpus", "steps", "warmup", "ms_per_step", "higher_is_better", "scaling", "vs_baseline", "dtype", "data",
+                     "config", "roofline", "cpu_baseline")
+
+
+def bench_line(out):
+    """The record as the ONE line on stdout: the headline's own fields whole, of each other leg its numbers, truth values and short texts (what lies deeper, and the
+    descriptions, are in the full record on stderr).  8 kB instead of 23: a log of which the last 20 kB are kept holds the whole line."""
+    def of_leg(leg):
+        if isinstance(leg, (list, tuple)):
+            return len(leg)
+        if isinstance(leg, dict):
+            return {k: v for k, v in leg.items() if not isinstance(v, (dict, list, tuple)) and not (isinstance(v, str) and len(v) > 60)}
+        return leg
+    return {k: v if k in WHOLE_IN_THE_LINE else of_leg(v) for k, v in out.items()}
 
 
 def secondary_summary(out):
