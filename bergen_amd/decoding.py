@@ -299,7 +299,8 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, scale=None, k_sca
     block_table [batch, width] int32: their pages in order.  A length is taken as 0 .. width * page_size, and the tokens of an entry
     outside the cache's pages are left out.  scale: 1 / sqrt(dim) unless given.  softcap c > 0: scores c tanh(s / c).  alibi_slopes [n_q]
     float32: minus slope times the distance.  window w > 0: the last w tokens only.  lse [batch, n_q] float32: log of the sum of e^score.
-    A sequence with nothing left gives zeros and -inf.
+    A sequence with nothing left gives zeros and -inf.  Scores, their sums and the outputs' are in 32 bits; weights are kept to 2^-17 of themselves (bf16 cache) or 2^-22 (fp16,
+    8-bit), where weights below 2^-39 of a head's largest are left out.
     """
     (pages, heads, page, dim), scaled = _cache_tensors(k_cache, v_cache, k_scale, v_scale)
     batch, nq, dim_q, q0, q1, qp = _rows("q", q)

@@ -371,6 +371,7 @@ int bh_op_qk_norm_rotary(const void* q, int64_t q_tok, int64_t q_head, void* q_o
  * = the least power of two >= 2^-126 with amax <= 448 * scale, code = x / scale rounded to nearest even.  A vector that holds an infinity or a NaN: scale = NaN, codes 0.
  * bh_op_kv_write: rows k, v [n_tokens][n_heads][head_dim] of dtype (fp16, bf16, fp32) go to their slots; a slot outside
  * [0, n_pages * page_size) is skipped.  Slots of one call must differ (of two rows with the same slot no whole vector need remain).
+ * The caches and scales must not share memory, nor be the memory of k and v where they are written.
  * bh_op_kv_read: the slots' vectors as dtype, code * scale rounded once; zeros for a slot outside the cache. */
 int bh_op_kv_write(const void* k, int64_t k_tok, int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, int32_t dtype,
                    const int64_t* slots, int64_t n_tokens, int32_t n_heads, int32_t head_dim, void* k_cache, void* v_cache, float* k_scale,
