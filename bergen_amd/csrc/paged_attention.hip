@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP == 256 ? 1 : DP == 64 ? 4 : EXA
                 float by = fade;
                 if constexpr (SCALED) {
                     slack *= fade;
-                    if (__any(slack < 0x1p-12f)) {  // (a large scale whose weight is gone must not hide the ones to come; 2^14 - 12 and hi + lo still keep 2^-27)
+                    if (__any(slack < 0x1p-12f)) {  // (a large scale whose weight is gone must not hide the ones to come; until then they are held times 2^2 and keep 2^-27)
                         const float to = fmaxf(LEAST, power_above(unit_v * slack));
                         by = unit_v * fade * over_power(0, to);  // at most 2^12: o is in 32 bits
                         unit_v = to, slack = 1.f;
